@@ -65,6 +65,16 @@ EXPORTS = [
     "gtmoe_weightfile_info",
     "gtmoe_weightfile_set_expert_layer",
     "gtmoe_weightfile_set_router",
+    "gtmoe_layer_norm",
+    "gtmoe_layer_norm_workspace",
+    "gtmoe_layer_norm_backward",
+    "gtmoe_dropout",
+    "gtmoe_dropout_backward",
+    "gtmoe_set_dropout",
+    "gtmoe_grouped_product",
+    "gtmoe_grouped_product_input_grad",
+    "gtmoe_grouped_product_weight_grad",
+    "gtmoe_operators_check",
 ]
 
 
@@ -144,6 +154,18 @@ def lib():
                                                 ctypes.POINTER(i64)]
             L.gtmoe_weightfile_set_expert_layer.argtypes = [vp, vp, i32, i32, i32, ctypes.c_char_p, ctypes.c_char_p]
             L.gtmoe_weightfile_set_router.argtypes = [vp, vp, ctypes.c_char_p, ctypes.c_char_p]
+            u64 = ctypes.c_uint64
+            L.gtmoe_layer_norm.argtypes = [vp, i32, i64, i64, vp, vp, i32, d, vp, vp, vp, vp]
+            L.gtmoe_layer_norm_workspace.argtypes = [i32, i64, i64, ctypes.POINTER(i64)]
+            L.gtmoe_layer_norm_backward.argtypes = [vp, vp, i32, i64, i64, vp, i32, vp, vp, vp, vp, vp, vp, i32, vp,
+                                                    i64, vp]
+            L.gtmoe_dropout.argtypes = [vp, vp, i32, i64, d, u64, u64, i64, vp, vp]
+            L.gtmoe_dropout_backward.argtypes = [vp, i32, i64, d, u64, u64, i64, vp, vp]
+            L.gtmoe_set_dropout.argtypes = [vp, d, u64, u64]
+            L.gtmoe_grouped_product.argtypes = [vp, vp, i32, i64, i64, i64, i32, vp, vp, vp]
+            L.gtmoe_grouped_product_input_grad.argtypes = [vp, vp, i32, i64, i64, i64, i32, vp, vp, vp]
+            L.gtmoe_grouped_product_weight_grad.argtypes = [vp, vp, i32, i64, i64, i64, i32, vp, vp, i32, i32, vp]
+            L.gtmoe_operators_check.argtypes = [i32]
             for name in EXPORTS:
                 if name not in ("gtmoe_destroy", "gtmoe_weightfile_close"):
                     fn = getattr(L, name)

@@ -659,7 +659,7 @@ void gtmoe_destroy(gtmoe_t h) {
                           &h->slot_row, &h->groups, &h->tile_prefix, &h->xp, &h->hp, &h->yp, &h->out_dev,
                           &h->res_dev, &h->fixups, &h->flagged, &h->x_pipe[0], &h->x_pipe[1], &h->out_pipe[0],
                           &h->out_pipe[1], &h->load_acc, &h->norm_w, &h->block_x, &h->block_xn,
-                          &h->block_xn16};
+                          &h->block_xn16, &h->block_xn16mid, &h->block_xn16lo, &h->block_y};
         for (DevBuf *b : bufs) b->release();
         release_training_state(h);
         for (cudaEvent_t e : h->pipe_ev)

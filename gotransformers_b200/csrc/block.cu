@@ -1,7 +1,7 @@
 // block.cu -- the mixture-of-experts half of a transformer block on the GPU:
 // out = x + MoE(RMSNorm(x)) (transformer.Block.Forward without hyper-
 // connections, transformer/block.go:72-77; dropout is the identity at
-// inference), so that a block's feed-forward step needs one call and no host
+// inference and applied when gtmoe_set_dropout gave a rate), so that a block's feed-forward step needs one call and no host
 // round trip between the norm, the mixture and the residual.
 //
 // RMSNorm.Forward (normalization/rmsnorm.go:33-53) is restated operation for
@@ -11,6 +11,7 @@
 // per element.  The normalized rows are the reference's bits, so routing on
 // them is exact as in gtmoe_forward.
 #include "handle.h"
+#include "operators.h"
 
 namespace gtmoe {
 namespace {
@@ -77,6 +78,16 @@ int gtmoe_set_norm(gtmoe_t h, const double *weights, double epsilon) {
     return 0;
 }
 
+int gtmoe_set_dropout(gtmoe_t h, double rate, uint64_t seed, uint64_t stream_id) {
+    if (!h) return fail(GTMOE_EINVAL, "handle is NULL");
+    GT_CHECK(check_dropout_rate(rate));
+    std::lock_guard<std::mutex> lock(h->mu);
+    h->drop_rate = rate;
+    h->drop_seed = seed;
+    h->drop_stream = stream_id;
+    return 0;
+}
+
 int gtmoe_forward_block(gtmoe_t h, const void *x, int x_dtype, int64_t T, const int64_t *token_ids, void *out,
                         int out_dtype, int32_t *chosen, double *gates, int32_t *perm, int64_t *load) {
     if (!h) return fail(GTMOE_EINVAL, "handle is NULL");
@@ -118,12 +129,25 @@ int gtmoe_forward_block(gtmoe_t h, const void *x, int x_dtype, int64_t T, const 
         h->gather_bf16 = h->block_xn16.p;
         h->router_bf16_mid = h->block_xn16mid.p;
         h->router_bf16_lo = h->block_xn16lo.p;
-        const int rc = forward_locked(h, h->block_xn.p, GTMOE_DTYPE_F64, T, token_ids, xd, out, out_dtype, chosen,
-                                      gates, perm, load);
+        // with dropout: the mixture's output as gtmoe_forward returns it, then
+        // one pass that drops and adds the residual
+        const bool drop = h->drop_rate > 0;
+        int rc = drop ? h->block_y.ensure(xbytes) : 0;
+        if (rc == 0)
+            rc = forward_locked(h, h->block_xn.p, GTMOE_DTYPE_F64, T, token_ids, drop ? nullptr : xd,
+                                drop ? h->block_y.p : out, out_dtype, chosen, gates, perm, load);
         h->gather_bf16 = nullptr;
         h->router_bf16_mid = nullptr;
         h->router_bf16_lo = nullptr;
-        return rc;
+        if (rc != 0 || !drop) return rc;
+        const bool out_dev = is_device_ptr(out);
+        void *od = out_dev ? out : h->block_y.p;
+        GT_CHECK(launch_dropout(h->block_y.p, xd, x_dtype, T * d, h->drop_rate, h->drop_seed, h->drop_stream, 0, od,
+                                h->stream));
+        if (out_dev) return 0;
+        GT_CUDA(cudaMemcpyAsync(out, od, xbytes, cudaMemcpyDeviceToHost, h->stream));
+        GT_CUDA(cudaStreamSynchronize(h->stream));
+        return tc_check_error(h->tc);
     }
 }
 

@@ -1,0 +1,195 @@
+// grouped_product.cu -- matrix products of rows grouped by expert, and the
+// gradients of both factors: the C entries, and the kernel on the SIMT cores
+// that takes every type, size and alignment.  bf16 operands that tile go to
+// the tensor cores (grouped_dense.cu).
+#include "grouped.h"
+
+namespace gtmoe {
+namespace {
+
+__device__ int g_error;  // first code a kernel recorded since the last check
+
+constexpr int kTile = 64;   // rows and columns of a block's tile
+constexpr int kStep = 16;   // terms of the sums per shared-memory step
+constexpr int kThreads = 256;
+
+// C[i][j] = sum over p of A(i, p) B(j, p):
+//   kProduct     i row, j output, p input:   A = X[i][p],  B = W_g[j][p]
+//   kInputGrad   i row, j input,  p output:  A = dY[i][p], B = W_g[p][j]
+//   kWeightGrad  i output, j input, p row:   A = dY[p][i], B = X[p][j]
+// 4 x 4 outputs per thread, each one sum in ascending p in ACC.
+template <typename T, typename ACC, typename OUT, GroupedOp OP>
+__global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const GroupedProduct a) {
+    __shared__ ACC sa[kStep][kTile + 4], sb[kStep][kTile + 4];
+    __shared__ int start[kMaxGroups + 1], tiles[kMaxGroups + 1], scratch[kThreads];
+    const bool ok = group_starts(a.counts, a.groups, a.rows, start, scratch);
+    if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_error, 0, kErrBadCounts);
+    const int64_t n_i = OP == kWeightGrad ? a.outputs : 0;
+    const int64_t n_j = OP == kProduct ? a.outputs : a.inputs;
+    const int64_t j_tiles = (n_j + kTile - 1) / kTile;
+    if (threadIdx.x == 0) {
+        int64_t n = 0;
+        for (int g = 0; g < a.groups; g++) {
+            tiles[g] = (int)n;
+            n += OP == kWeightGrad ? (n_i + kTile - 1) / kTile : (start[g + 1] - start[g] + kTile - 1) / kTile;
+        }
+        tiles[a.groups] = (int)n;
+    }
+    __syncthreads();
+    const int64_t total = (int64_t)tiles[a.groups] * j_tiles;
+    const T *A = (const T *)a.a, *B = (const T *)a.b;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    int g = 0;
+    for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
+        const int it = (int)(u / j_tiles);
+        while (tiles[g + 1] <= it) g++;
+        const int64_t i0 = (int64_t)(it - tiles[g]) * kTile, j0 = (u % j_tiles) * kTile;
+        const int64_t r0 = start[g], m = start[g + 1] - start[g];
+        const int64_t i_end = OP == kWeightGrad ? n_i : m;
+        const int64_t p_end = OP == kProduct ? a.inputs : OP == kInputGrad ? a.outputs : m;
+        const T *Wg = B + (int64_t)g * a.outputs * a.inputs;
+        ACC acc[4][4] = {};
+        for (int64_t p0 = 0; p0 < p_end; p0 += kStep) {
+            // consecutive threads along the operand's contiguous axis
+#pragma unroll
+            for (int q = 0; q < kTile * kStep / kThreads; q++) {
+                const int e = q * kThreads + threadIdx.x;
+                const int ap = OP == kWeightGrad ? e / kTile : e % kStep, ai = OP == kWeightGrad ? e % kTile : e / kStep;
+                const int bp = OP == kProduct ? e % kStep : e / kTile, bj = OP == kProduct ? e / kStep : e % kTile;
+                ACC va = ACC(0), vb = ACC(0);
+                if (i0 + ai < i_end && p0 + ap < p_end)
+                    va = (ACC)(OP == kWeightGrad ? A[(r0 + p0 + ap) * a.outputs + i0 + ai]
+                                                 : A[(r0 + i0 + ai) * (OP == kProduct ? a.inputs : a.outputs) + p0 + ap]);
+                if (j0 + bj < n_j && p0 + bp < p_end)
+                    vb = (ACC)(OP == kProduct      ? Wg[(j0 + bj) * a.inputs + p0 + bp]
+                               : OP == kInputGrad ? Wg[(p0 + bp) * a.inputs + j0 + bj]
+                                                  : B[(r0 + p0 + bp) * a.inputs + j0 + bj]);
+                sa[ap][ai] = va;
+                sb[bp][bj] = vb;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < kStep; p++) {
+                ACC ra[4], rb[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    ra[q] = sa[p][ty * 4 + q];
+                    rb[q] = sb[p][tx * 4 + q];
+                }
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) acc[x][y] += ra[x] * rb[y];
+            }
+            __syncthreads();
+        }
+        OUT *C = (OUT *)a.c;
+        const int64_t base = OP == kWeightGrad ? (int64_t)g * a.outputs * a.inputs : r0 * n_j;
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const int64_t i = i0 + ty * 4 + x, j = j0 + tx * 4 + y;
+                if (i < i_end && j < n_j) {
+                    OUT &o = C[base + i * n_j + j];
+                    o = (OUT)(OP == kWeightGrad && a.accumulate ? (ACC)o + acc[x][y] : acc[x][y]);
+                }
+            }
+    }
+}
+
+template <typename T, typename ACC, typename OUT, GroupedOp OP>
+int launch_simt(const GroupedProduct &p, cudaStream_t st) {
+    const int64_t n_j = OP == kProduct ? p.outputs : p.inputs;
+    // at most this many tiles: the rows of a group end inside a tile
+    const int64_t i_tiles = OP == kWeightGrad ? (int64_t)p.groups * ((p.outputs + kTile - 1) / kTile)
+                                              : p.rows / kTile + (p.rows < p.groups ? p.rows : p.groups);
+    const int64_t most = i_tiles * ((n_j + kTile - 1) / kTile);
+    const unsigned grid = (unsigned)(most < 148 * 16 ? most : 148 * 16);
+    grouped_simt_product_kernel<T, ACC, OUT, OP><<<grid, kThreads, 0, st>>>(p);
+    GT_CUDA(cudaGetLastError());
+    note_launches(1);
+    return 0;
+}
+
+template <typename T, typename ACC>
+int launch_simt_op(const GroupedProduct &p, cudaStream_t st) {
+    if (p.op == kProduct) return launch_simt<T, ACC, T, kProduct>(p, st);
+    if (p.op == kInputGrad) return launch_simt<T, ACC, T, kInputGrad>(p, st);
+    if (p.out_dtype == p.dtype) return launch_simt<T, ACC, T, kWeightGrad>(p, st);
+    return launch_simt<T, ACC, float, kWeightGrad>(p, st);
+}
+
+int run_grouped(const GroupedProduct &p, const char *a_name, const char *b_name, const char *c_name, void *stream) {
+    if (!known_dtype(p.dtype) || !known_dtype(p.out_dtype)) return fail(GTMOE_EINVAL, "grouped product: unknown dtype");
+    if (p.out_dtype != p.dtype && !(p.dtype == GTMOE_DTYPE_BF16 && p.out_dtype == GTMOE_DTYPE_F32))
+        return fail(GTMOE_EINVAL, "grouped product: weight gradients have the operands' dtype, or float32 beside bfloat16");
+    if (p.rows < 0 || p.rows > 0x7fffff00)
+        return fail(GTMOE_EINVAL, "grouped product: rows must be between 0 and 2^31 - 256, got %lld", (long long)p.rows);
+    if (p.inputs < 1 || p.outputs < 1 || p.inputs > 0x7fffff00 || p.outputs > 0x7fffff00)
+        return fail(GTMOE_EINVAL, "grouped product: inputs and outputs must be between 1 and 2^31 - 256, got %lld and %lld",
+                    (long long)p.inputs, (long long)p.outputs);
+    if (p.groups < 1 || p.groups > kMaxGroups)
+        return fail(GTMOE_EINVAL, "grouped product: needs 1 to %d groups, got %d", kMaxGroups, p.groups);
+    if (!countable(p.rows, p.inputs) || !countable(p.rows, p.outputs) || !countable(p.inputs * p.groups, p.outputs))
+        return fail(GTMOE_EINVAL, "grouped product: an operand is too large");
+    if ((p.outputs + kTile - 1) / kTile * p.groups > 0x7fffffff)
+        return fail(GTMOE_EINVAL, "grouped product: too many outputs for %d groups", p.groups);
+    if (p.rows == 0 && p.op != kWeightGrad) return 0;
+    if (p.rows == 0 && p.accumulate) return 0;
+    if ((p.rows > 0 && (!p.a || !p.b)) || !p.c || !p.counts)
+        return fail(GTMOE_EINVAL, "grouped product: %s, %s, counts and %s must be given", a_name, b_name, c_name);
+    const int64_t es = (int64_t)dtype_size(p.dtype);
+    const int64_t xb = p.rows * p.inputs * es, yb = p.rows * p.outputs * es;
+    const int64_t wn = p.groups * p.inputs * p.outputs;
+    const int64_t ab = p.op == kProduct ? xb : yb, bb = p.op == kWeightGrad ? xb : wn * es;
+    const int64_t cb = p.op == kProduct     ? yb
+                       : p.op == kInputGrad ? xb
+                                            : wn * (int64_t)dtype_size(p.out_dtype);
+    if (ranges_overlap(p.c, cb, p.a, ab) || ranges_overlap(p.c, cb, p.b, bb) || ranges_overlap(p.c, cb, p.counts, 8 * (int64_t)p.groups))
+        return fail(GTMOE_EINVAL, "grouped product: %s overlaps another argument", c_name);
+    DeviceScope scope;
+    GT_CHECK(scope.enter({{p.c, c_name, dtype_size(p.out_dtype)}, {ab ? p.a : nullptr, a_name, (size_t)es},
+                          {bb ? p.b : nullptr, b_name, (size_t)es}, {p.counts, "counts", 8}}));
+    cudaStream_t st = (cudaStream_t)stream;
+    if (p.dtype == GTMOE_DTYPE_F64) return launch_simt_op<double, double>(p, st);
+    if (p.dtype == GTMOE_DTYPE_F32) return launch_simt_op<float, float>(p, st);
+    return launch_simt_op<__nv_bfloat16, float>(p, st);
+}
+
+}  // namespace
+
+int grouped_take_error(int *code) {
+    GT_CUDA(cudaDeviceSynchronize());
+    const int zero = 0;
+    GT_CUDA(cudaMemcpyFromSymbol(code, g_error, sizeof(int)));
+    if (*code) GT_CUDA(cudaMemcpyToSymbol(g_error, &zero, sizeof(int)));
+    return 0;
+}
+
+}  // namespace gtmoe
+
+using namespace gtmoe;
+
+extern "C" {
+
+int gtmoe_grouped_product(const void *x, const void *w, int dtype, int64_t rows, int64_t inputs, int64_t outputs,
+                          int groups, const int64_t *counts, void *y, void *stream) {
+    const GroupedProduct p = {kProduct, dtype, dtype, 0, rows, inputs, outputs, groups, counts, x, w, y};
+    return run_grouped(p, "x", "w", "y", stream);
+}
+
+int gtmoe_grouped_product_input_grad(const void *dy, const void *w, int dtype, int64_t rows, int64_t inputs,
+                                     int64_t outputs, int groups, const int64_t *counts, void *dx, void *stream) {
+    const GroupedProduct p = {kInputGrad, dtype, dtype, 0, rows, inputs, outputs, groups, counts, dy, w, dx};
+    return run_grouped(p, "dy", "w", "dx", stream);
+}
+
+int gtmoe_grouped_product_weight_grad(const void *dy, const void *x, int dtype, int64_t rows, int64_t inputs,
+                                      int64_t outputs, int groups, const int64_t *counts, void *dw, int dw_dtype,
+                                      int accumulate, void *stream) {
+    const GroupedProduct p = {kWeightGrad, dtype, dw_dtype, accumulate, rows, inputs, outputs, groups, counts, dy, x, dw};
+    return run_grouped(p, "dy", "x", "dw", stream);
+}
+
+}  // extern "C"

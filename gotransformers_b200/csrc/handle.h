@@ -119,6 +119,11 @@ struct gtmoe_handle {
     const void *router_bf16_lo = nullptr;
     double norm_eps = 0;
     int norm_set = 0;
+    // the block's dropout (gtmoe_set_dropout), and the mixture's output
+    // before it
+    double drop_rate = 0;
+    uint64_t drop_seed = 0, drop_stream = 0;
+    DevBuf block_y;
 
     // training (backward.cu): what gtmoe_backward needs from the last Forward
     // (its input rows as float64, chosen experts, gates, the expert-sorted

@@ -20,6 +20,16 @@ import numpy as np
 
 from . import _lib
 from ._lib import DOWN, DTYPE_BF16, DTYPE_F32, DTYPE_F64, FLOAT32, FLOAT64, FP4, GATE, INT8, ROUTED, SHARED, UP, check
+from .operators import (
+    check_operators,
+    dropout,
+    dropout_backward,
+    grouped_product,
+    grouped_product_input_gradients,
+    grouped_product_weight_gradients,
+    layer_norm,
+    layer_norm_backward,
+)
 
 
 def _addr(a):
@@ -275,6 +285,12 @@ class MixtureOfExperts:
             self.last_rows_for_expert = perm
         return out
 
+    def set_dropout(self, rate: float, seed: int = 0, stream: int = 0):
+        """Dropout of the mixture's output inside forward_block: x +
+        dropout(Forward(RMSNorm(x))) from now on, with dropout()'s decisions
+        for (rate, seed, stream); rate 0 switches it off."""
+        check(_lib.lib().gtmoe_set_dropout(self._h, float(rate), seed, stream))
+
     # -- training
     def set_training(self, on: bool = True):
         """Keep, from every later forward, what backward() needs."""
@@ -365,6 +381,14 @@ __all__ = [
     "quantize_rows",
     "fill_normal",
     "WeightFile",
+    "layer_norm",
+    "layer_norm_backward",
+    "dropout",
+    "dropout_backward",
+    "grouped_product",
+    "grouped_product_input_gradients",
+    "grouped_product_weight_gradients",
+    "check_operators",
     "FLOAT64",
     "FLOAT32",
     "INT8",

@@ -293,6 +293,101 @@ GTMOE_API int gtmoe_read_timing(gtmoe_t h, double *ms, int n_phases, int64_t *ca
 GTMOE_API int gtmoe_route_noalloc(gtmoe_t h, const void *x, int x_dtype, int64_t T, const int64_t *token_ids,
                                   int32_t *chosen, double *gates);
 
+/* ---- Operators without a handle, for training a block around or with its
+ * experts.  Conventions of this section:
+ *  - Every pointer is device memory (or managed memory) of one device, dense
+ *    and row-major, aligned to its elements; the call runs on that device
+ *    whatever the calling thread's current one is, and leaves that as it was.
+ *  - `stream` is a cudaStream_t of that device (NULL = its default stream).
+ *    The calls are asynchronous, allocate nothing, keep nothing between calls
+ *    and may be captured into CUDA graphs; any thread may make them at once.
+ *  - Workspaces are the caller's, at least as large as the matching
+ *    _workspace call says and 16-byte aligned; calls that may run at the same
+ *    time need one each.
+ *  - Where an output may be one of the inputs, that is said; other overlaps,
+ *    host memory, unknown dtypes and impossible sizes are GTMOE_EINVAL.
+ *  - Results do not depend on the run: every sum has a fixed order. */
+
+/* Layer norm of rows (rows x width): y = (x - mean) * rstd * weight + bias
+ * with rstd = 1 / sqrt(mean((x - mean)^2) + epsilon); the counterpart of
+ * gtmoe_forward_block's RMSNorm (normalization/rmsnorm.go:33-53) for blocks
+ * that centre their rows.  weight and bias (width values each) may be NULL (1
+ * and 0) and have the rows' dtype, or float32 beside bfloat16 rows.  mean and
+ * rstd (rows values each, float32, float64 for float64 rows; NULL to skip)
+ * are what the backward needs.  Sums are float32 (float64 for float64 rows).
+ * y may be x. */
+GTMOE_API int gtmoe_layer_norm(const void *x, int dtype, int64_t rows, int64_t width, const void *weight,
+                     const void *bias, int weight_dtype, double epsilon, void *y, void *mean, void *rstd,
+                     void *stream);
+
+/* Its backward pass: with g = dy * weight and xh = (x - mean) * rstd,
+ *   dx      = rstd * (g - mean(g) - xh * mean(g * xh)) [+ dresidual]
+ *   dweight = sum over rows of dy * xh,   dbias = sum over rows of dy
+ * (both in weight_dtype; NULL to skip; accumulate != 0 adds to them, as
+ * gtmoe_backward adds the router's gradients).  dresidual (rows x width, NULL
+ * for none) is the gradient that reaches x beside the norm, such as that of
+ * the block's residual.  dx may be dy, x or dresidual.  The workspace is
+ * needed for dweight and dbias only. */
+GTMOE_API int gtmoe_layer_norm_workspace(int dtype, int64_t rows, int64_t width, int64_t *bytes);
+GTMOE_API int gtmoe_layer_norm_backward(const void *dy, const void *x, int dtype, int64_t rows, int64_t width,
+                              const void *weight, int weight_dtype, const void *mean, const void *rstd,
+                              const void *dresidual, void *dx, void *dweight, void *dbias, int accumulate,
+                              void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Dropout (the block's FeedForwardDropout, transformer/block.go:76) with the
+ * residual of block.go:77: out[i] = residual[i] + (keep(i) ? x[i] / (1 - rate)
+ * : 0) over n values; residual may be NULL.  A dropped value does not reach
+ * the output, whatever it is.  No mask is stored: keep(i) depends on seed,
+ * stream_id and offset + i alone.  Word j of a stream is SplitMix64(key + j),
+ * key = SplitMix64(seed ^ (stream_id * 0xD1B54A32D192ED03)) as in
+ * gtmoe_fill_normal; element e owns the low (e even) or high (e odd) 32 bits
+ * of word e / 2 and is kept when they are at least floor(rate * 2^32), 0 <=
+ * rate < 1.  offset lets a part of a batch make the whole batch's decisions.
+ * out may be x or residual. */
+GTMOE_API int gtmoe_dropout(const void *x, const void *residual, int dtype, int64_t n, double rate, uint64_t seed,
+                  uint64_t stream_id, int64_t offset, void *out, void *stream);
+/* dx[i] = keep(i) ? dout[i] / (1 - rate) : 0; the residual's gradient is dout
+ * itself.  dx may be dout. */
+GTMOE_API int gtmoe_dropout_backward(const void *dout, int dtype, int64_t n, double rate, uint64_t seed,
+                           uint64_t stream_id, int64_t offset, void *dx, void *stream);
+/* Dropout inside gtmoe_forward_block: out = x + dropout(Forward(RMSNorm(x)))
+ * from now on, with the decisions of gtmoe_dropout over the T x d values at
+ * offset 0.  A training step gives every step its own stream_id; rate 0 (the
+ * start) switches it off.  The gradient of the mixture's output, which
+ * gtmoe_backward takes, is then gtmoe_dropout_backward's. */
+GTMOE_API int gtmoe_set_dropout(gtmoe_t h, double rate, uint64_t seed, uint64_t stream_id);
+
+/* Matrix products of rows sorted by expert with dense expert weights, the
+ * trainable counterpart of the expert layers that a handle keeps compressed
+ * (perceptron.Layer, perceptron/layer.go:133-162, once per expert).  Group g
+ * has counts[g] consecutive rows after those of the groups before it (the
+ * layout and the counts of gtmoe_forward's perm and load); w is groups x
+ * outputs x inputs.
+ *   y[r]  = x[r] w_g^T         x rows x inputs, y rows x outputs
+ *   dx[r] = dy[r] w_g
+ *   dw_g  = sum over g's rows of dy[r]^T x[r]; in dtype, or float32 beside
+ *           bfloat16; zeros for a group without rows; accumulate != 0 adds
+ * All operands have one dtype; sums are float32 (float64 for float64).  At
+ * most 1024 groups and 2^31 - 256 rows.  counts is device memory, so no call
+ * waits for the host.  Rows after the last group's are neither read nor
+ * written.  A negative count (taken as 0) or a sum above `rows` (rows past the
+ * end left out) is reported by gtmoe_operators_check.  No output may be an
+ * input.  bfloat16 operands with inputs and outputs a multiple of 8 that
+ * start on 16 bytes run on the tensor cores. */
+GTMOE_API int gtmoe_grouped_product(const void *x, const void *w, int dtype, int64_t rows, int64_t inputs,
+                          int64_t outputs, int groups, const int64_t *counts, void *y, void *stream);
+GTMOE_API int gtmoe_grouped_product_input_grad(const void *dy, const void *w, int dtype, int64_t rows, int64_t inputs,
+                                     int64_t outputs, int groups, const int64_t *counts, void *dx, void *stream);
+GTMOE_API int gtmoe_grouped_product_weight_grad(const void *dy, const void *x, int dtype, int64_t rows,
+                                      int64_t inputs, int64_t outputs, int groups, const int64_t *counts, void *dw,
+                                      int dw_dtype, int accumulate, void *stream);
+
+/* What the grouped products' kernels recorded on `device` since the last
+ * check: waits for the device, then 0, GTMOE_EINVAL (refused counts) or
+ * GTMOE_ETIMEOUT (a bounded wait ran out); the record is cleared.  Not inside
+ * a stream capture. */
+GTMOE_API int gtmoe_operators_check(int device);
+
 /* The library's failure path on a device, without a fault; no counterpart in
  * the reference.  Every device-side wait of this library is bounded (2 s of
  * %globaltimer): on expiry the kernel records an error code, stops and
