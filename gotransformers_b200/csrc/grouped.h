@@ -29,54 +29,71 @@ struct GroupedProduct {
 
 constexpr int kMaxGroups = kMaxRoutedExperts;
 
+// Inclusive scan of one value per thread of the block over the threads, cut at
+// `most` (< 2^31; cutting a sum of non-negative values early or late gives the
+// same).  `scratch` is one word per thread; returns the threads' sum before
+// this one's.
+__device__ __forceinline__ int64_t block_scan(int64_t own, int64_t most, int *scratch) {
+    const int t = threadIdx.x;
+    scratch[t] = (int)(own < most ? own : most);
+    __syncthreads();
+    for (int o = 1; o < (int)blockDim.x; o <<= 1) {
+        const int64_t v = (int64_t)scratch[t] + (t >= o ? scratch[t - o] : 0);
+        __syncthreads();
+        scratch[t] = (int)(v < most ? v : most);
+        __syncthreads();
+    }
+    return t ? scratch[t - 1] : 0;
+}
+
 // Group g's rows are start[g] .. start[g + 1], cut at `rows`; a negative
-// count is no rows.  Every thread of the block calls it; `start` is groups + 1
-// words of shared memory and `scratch` one word per thread.  True when the
-// counts were as they should be.
-__device__ __forceinline__ bool group_starts(const int64_t *__restrict__ counts, int groups, int64_t rows, int *start,
-                                             int *scratch) {
+// count is no rows.  tiles[g] is the number of tiles before group g, of
+// tile_rows rows each, or with tile_rows = 0 of per_group for every group.
+// Every thread of the block calls it; start and tiles are groups + 1 words of
+// shared memory, scratch one word per thread.  True when the counts were as
+// they should be.
+__device__ __forceinline__ bool group_ranges(const int64_t *__restrict__ counts, int groups, int64_t rows,
+                                             int tile_rows, int per_group, int *start, int *tiles, int *scratch) {
     const int threads = blockDim.x, t = threadIdx.x;
     const int per = (groups + threads - 1) / threads;
-    const int g0 = t * per, g1 = min(groups, g0 + per);
+    const int g0 = min(groups, t * per), g1 = min(groups, g0 + per);
     int64_t sum = 0;
     bool ok = true;
     for (int g = g0; g < g1; g++) {
         int64_t c = counts[g];
-        if (c < 0 || c > rows) {
-            ok = false;
-            c = c < 0 ? 0 : rows;
-        }
+        ok = ok && c >= 0 && c <= rows;
+        c = c < 0 ? 0 : c < rows ? c : rows;
         sum += c;
-        if (sum > rows) {
-            ok = false;
-            sum = rows;
-        }
         start[g + 1] = (int)c;
     }
-    scratch[t] = (int)sum;
-    __syncthreads();
-    // inclusive scan over the threads, saturating at `rows` (< 2^31)
-    for (int o = 1; o < threads; o <<= 1) {
-        const int64_t add = t >= o ? (int64_t)scratch[t - o] : 0;
-        __syncthreads();
-        const int64_t v = (int64_t)scratch[t] + add;
-        if (v > rows) ok = false;
-        scratch[t] = (int)(v > rows ? rows : v);
-        __syncthreads();
-    }
-    int64_t at = t ? scratch[t - 1] : 0;
+    // one more than `rows` still tells a sum that is too large
+    int64_t at = block_scan(sum, rows + 1, scratch);
+    ok = ok && at + sum <= rows;
+    int64_t n_tiles = 0;
     for (int g = g0; g < g1; g++) {
+        const int64_t first = at < rows ? at : rows;
         at += start[g + 1];
-        if (at > rows) at = rows;
-        start[g + 1] = (int)at;
+        const int64_t last = at < rows ? at : rows;
+        start[g + 1] = (int)last;
+        const int64_t n = tile_rows ? (last - first + tile_rows - 1) / tile_rows : per_group;
+        n_tiles += n;
+        tiles[g + 1] = (int)n;
     }
-    if (t == 0) start[0] = 0;
+    __syncthreads();
+    at = block_scan(n_tiles, 0x7ffffffe, scratch);
+    for (int g = g0; g < g1; g++) {
+        at += tiles[g + 1];
+        tiles[g + 1] = (int)at;
+    }
+    if (t == 0) start[0] = tiles[0] = 0;
     return __syncthreads_and(ok);
 }
 
 // The tensor-core kernel, and whether it takes these sizes, types and
 // addresses.
 bool grouped_dense_usable(const GroupedProduct &p);
-int launch_grouped_dense(const GroupedProduct &p, int *err, cudaStream_t st);
+int launch_grouped_dense(const GroupedProduct &p, int device, cudaStream_t st);
+// Reads and clears the code that kernel recorded on the current device.
+int grouped_dense_take_error(int *code);
 
 }  // namespace gtmoe

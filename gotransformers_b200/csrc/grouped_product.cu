@@ -22,20 +22,11 @@ template <typename T, typename ACC, typename OUT, GroupedOp OP>
 __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const GroupedProduct a) {
     __shared__ ACC sa[kStep][kTile + 4], sb[kStep][kTile + 4];
     __shared__ int start[kMaxGroups + 1], tiles[kMaxGroups + 1], scratch[kThreads];
-    const bool ok = group_starts(a.counts, a.groups, a.rows, start, scratch);
-    if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_error, 0, kErrBadCounts);
-    const int64_t n_i = OP == kWeightGrad ? a.outputs : 0;
     const int64_t n_j = OP == kProduct ? a.outputs : a.inputs;
     const int64_t j_tiles = (n_j + kTile - 1) / kTile;
-    if (threadIdx.x == 0) {
-        int64_t n = 0;
-        for (int g = 0; g < a.groups; g++) {
-            tiles[g] = (int)n;
-            n += OP == kWeightGrad ? (n_i + kTile - 1) / kTile : (start[g + 1] - start[g] + kTile - 1) / kTile;
-        }
-        tiles[a.groups] = (int)n;
-    }
-    __syncthreads();
+    const bool ok = group_ranges(a.counts, a.groups, a.rows, OP == kWeightGrad ? 0 : kTile,
+                                 (int)((a.outputs + kTile - 1) / kTile), start, tiles, scratch);
+    if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_error, 0, kErrBadCounts);
     const int64_t total = (int64_t)tiles[a.groups] * j_tiles;
     const T *A = (const T *)a.a, *B = (const T *)a.b;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -45,7 +36,7 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
         while (tiles[g + 1] <= it) g++;
         const int64_t i0 = (int64_t)(it - tiles[g]) * kTile, j0 = (u % j_tiles) * kTile;
         const int64_t r0 = start[g], m = start[g + 1] - start[g];
-        const int64_t i_end = OP == kWeightGrad ? n_i : m;
+        const int64_t i_end = OP == kWeightGrad ? a.outputs : m;
         const int64_t p_end = OP == kProduct ? a.inputs : OP == kInputGrad ? a.outputs : m;
         const T *Wg = B + (int64_t)g * a.outputs * a.inputs;
         ACC acc[4][4] = {};
@@ -152,6 +143,7 @@ int run_grouped(const GroupedProduct &p, const char *a_name, const char *b_name,
     GT_CHECK(scope.enter({{p.c, c_name, dtype_size(p.out_dtype)}, {ab ? p.a : nullptr, a_name, (size_t)es},
                           {bb ? p.b : nullptr, b_name, (size_t)es}, {p.counts, "counts", 8}}));
     cudaStream_t st = (cudaStream_t)stream;
+    if (grouped_dense_usable(p)) return launch_grouped_dense(p, scope.device(), st);
     if (p.dtype == GTMOE_DTYPE_F64) return launch_simt_op<double, double>(p, st);
     if (p.dtype == GTMOE_DTYPE_F32) return launch_simt_op<float, float>(p, st);
     return launch_simt_op<__nv_bfloat16, float>(p, st);
@@ -161,9 +153,13 @@ int run_grouped(const GroupedProduct &p, const char *a_name, const char *b_name,
 
 int grouped_take_error(int *code) {
     GT_CUDA(cudaDeviceSynchronize());
+    int simt = 0, dense = 0;
     const int zero = 0;
-    GT_CUDA(cudaMemcpyFromSymbol(code, g_error, sizeof(int)));
-    if (*code) GT_CUDA(cudaMemcpyToSymbol(g_error, &zero, sizeof(int)));
+    GT_CUDA(cudaMemcpyFromSymbol(&simt, g_error, sizeof(int)));
+    if (simt) GT_CUDA(cudaMemcpyToSymbol(g_error, &zero, sizeof(int)));
+    GT_CHECK(grouped_dense_take_error(&dense));
+    // an expired wait before refused counts
+    *code = dense && dense != kErrBadCounts ? dense : simt ? simt : dense;
     return 0;
 }
 
