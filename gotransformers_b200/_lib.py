@@ -73,6 +73,7 @@ EXPORTS = [
     "gtmoe_set_dropout",
     "gtmoe_grouped_product",
     "gtmoe_grouped_product_input_grad",
+    "gtmoe_grouped_product_workspace",
     "gtmoe_grouped_product_weight_grad",
     "gtmoe_operators_check",
 ]
@@ -164,7 +165,9 @@ def lib():
             L.gtmoe_set_dropout.argtypes = [vp, d, u64, u64]
             L.gtmoe_grouped_product.argtypes = [vp, vp, i32, i64, i64, i64, i32, vp, vp, vp]
             L.gtmoe_grouped_product_input_grad.argtypes = [vp, vp, i32, i64, i64, i64, i32, vp, vp, vp]
-            L.gtmoe_grouped_product_weight_grad.argtypes = [vp, vp, i32, i64, i64, i64, i32, vp, vp, i32, i32, vp]
+            L.gtmoe_grouped_product_weight_grad.argtypes = [vp, vp, i32, i64, i64, i64, i32, vp, vp, i32, i32, vp,
+                                                            i64, vp]
+            L.gtmoe_grouped_product_workspace.argtypes = [i32, i64, i64, i64, i32, ctypes.POINTER(i64)]
             L.gtmoe_operators_check.argtypes = [i32]
             for name in EXPORTS:
                 if name not in ("gtmoe_destroy", "gtmoe_weightfile_close"):

@@ -25,9 +25,11 @@ struct GroupedProduct {
     const void *a;    // X, dY, dY
     const void *b;    // W, W, X
     void *c;          // Y, dX, dW
+    void *workspace;  // kWeightGrad: grouped_dense_workspace() bytes
 };
 
 constexpr int kMaxGroups = kMaxRoutedExperts;
+constexpr int kAnyRows = 0x7fffffff;  // a tile_rows that no group fills
 
 // Inclusive scan of one value per thread of the block over the threads, cut at
 // `most` (< 2^31; cutting a sum of non-negative values early or late gives the
@@ -47,16 +49,17 @@ __device__ __forceinline__ int64_t block_scan(int64_t own, int64_t most, int *sc
 }
 
 // Group g's rows are start[g] .. start[g + 1], cut at `rows`; a negative
-// count is no rows.  tiles[g] is the number of tiles before group g, of
-// tile_rows rows each, or with tile_rows = 0 of per_group for every group.
-// Every thread of the block calls it; start and tiles are groups + 1 words of
-// shared memory, scratch one word per thread.  True when the counts were as
-// they should be.
+// count is no rows.  tiles[g] is the number of tiles before group g: `per` for
+// each run of tile_rows rows that it has begun, of which it has at least
+// `least`.  Every thread of the block calls it; start and tiles are groups + 1
+// words of shared memory, scratch one word per thread.  True when the counts
+// were as they should be.
 __device__ __forceinline__ bool group_ranges(const int64_t *__restrict__ counts, int groups, int64_t rows,
-                                             int tile_rows, int per_group, int *start, int *tiles, int *scratch) {
+                                             int tile_rows, int least, int per, int *start, int *tiles,
+                                             int *scratch) {
     const int threads = blockDim.x, t = threadIdx.x;
-    const int per = (groups + threads - 1) / threads;
-    const int g0 = min(groups, t * per), g1 = min(groups, g0 + per);
+    const int run = (groups + threads - 1) / threads;
+    const int g0 = min(groups, t * run), g1 = min(groups, g0 + run);
     int64_t sum = 0;
     bool ok = true;
     for (int g = g0; g < g1; g++) {
@@ -75,7 +78,8 @@ __device__ __forceinline__ bool group_ranges(const int64_t *__restrict__ counts,
         at += start[g + 1];
         const int64_t last = at < rows ? at : rows;
         start[g + 1] = (int)last;
-        const int64_t n = tile_rows ? (last - first + tile_rows - 1) / tile_rows : per_group;
+        const int64_t begun = (last - first + tile_rows - 1) / tile_rows;
+        const int64_t n = per * (begun < least ? least : begun);
         n_tiles += n;
         tiles[g + 1] = (int)n;
     }
@@ -95,5 +99,7 @@ bool grouped_dense_usable(const GroupedProduct &p);
 int launch_grouped_dense(const GroupedProduct &p, int device, cudaStream_t st);
 // Reads and clears the code that kernel recorded on the current device.
 int grouped_dense_take_error(int *code);
+// Bytes of workspace of its weight gradient (0 unless the sums are split).
+int64_t grouped_dense_workspace(int64_t rows, int64_t inputs, int64_t outputs, int groups);
 
 }  // namespace gtmoe

@@ -17,16 +17,28 @@
 // SBO = 8 rows of the sum).
 //
 // Each CTA stages its 128 rows of A and its half of B in shared memory by TMA
-// (64 terms of the sum per stage, 128-byte swizzle).  Terms past the end of
-// the sum's axis are read as zeros by TMA, from a three-dimensional view of
-// the weights, so that the next group's weights are never multiplied.  The
-// sum over rows ends inside a stage: there a warp of each CTA zeroes the rows
-// past the group's end of both operands before the MMA (0 * NaN is NaN, so
-// one operand would not do).
+// (64 terms of the sum per stage, 128-byte swizzle), one TMA instruction per
+// operand: a CTA issues one per about 200 clocks whatever its size, so that a
+// stage of four 8 KB boxes took 826 clocks where the MMAs need 512.  An M- or
+// N-major operand is therefore viewed as 64-column chunks x rows, two chunks to
+// a box, except where a chunk is cut by the operand's last column.  Terms past
+// the end of the sum's axis are read as zeros by TMA, from a view of the
+// weights with an axis for the groups, so that the next group's weights are
+// never multiplied.  The sum over rows ends inside a stage: there a warp of
+// each CTA zeroes the rows past the group's end of both operands before the MMA
+// (0 * NaN is NaN, so one operand would not do).
+//
+// The tensor cores cut every addition to an accumulator towards zero: over n
+// rows the sums shrink by about n / 16 * 2^-24.2 (measured: 4.0e-7 at 512 rows,
+// 6.6e-5 at 65536), far more than float32 rounding.  The weight gradient,
+// whose result may be float32 and whose sums are the long ones, is therefore
+// accumulated in runs of kRunStages stages; the epilogue adds the runs in
+// registers, with rounding, while the next run is multiplied.  Results in bf16
+// keep one sum: their rounding is 2^-9.
 //
 // Persistent kernel, one CTA per SM; warp 0 TMA, warp 1 MMA issue (leader),
-// warps 2-5 epilogue (TMEM -> bf16 / float32 -> shared memory -> coalesced
-// rows), warp 6 zeroes row tails.  Two accumulators: the epilogue of a tile
+// warps 2-9 epilogue (TMEM -> bf16 / float32 -> shared memory -> coalesced
+// rows), warp 10 zeroes row tails.  Two accumulators: the epilogue of a tile
 // overlaps the next tile's products.  Every wait is bounded as in tc.cu.
 #include <atomic>
 
@@ -39,24 +51,25 @@ namespace {
 __device__ int g_dense_error;
 
 constexpr int kStageK = 64;              // terms of the sum per stage
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kHalf = 128;               // rows of A, and most rows of B, per CTA
 constexpr int kTileM = 2 * kHalf, kTileN = 2 * kHalf;
 constexpr int kOperandBytes = kHalf * kStageK * 2;  // 16 KB
 constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kSmallBox = 32;            // rows of a TMA box of a partial tile of B
+constexpr int kRunStages = 8;            // stages of the weight gradient's sums per run (512 rows)
 constexpr int kChunkBytes = kStageK * 128;  // 64 columns x 64 terms of an M- or N-major operand
-constexpr int kEpiWarps = 4;
-constexpr int kThreads = 7 * 32;
+constexpr int kEpiWarps = 8;             // two groups of four (one per TMEM lane quadrant), half the columns each
+constexpr int kThreads = (3 + kEpiWarps) * 32;
 constexpr int kTmemCols = 512;
-constexpr int kBandTiles = 16;           // row tiles per band of the unit order
-// epilogue staging: two buffers of 32 rows x 128 bf16 (pitch 272 bytes), or
-// per warp 32 rows x 32 float32 (pitch 144 bytes)
+constexpr int kBandTiles = 8;            // row tiles per band of the unit order
+// epilogue staging, per group of warps two buffers of 16 rows x 128 bf16
+// (pitch 272 bytes), or per warp 32 rows x 32 float32 (pitch 144 bytes)
+constexpr int kChunkRows = 16;
 constexpr int kRowPitch = 272;
-constexpr int kRowBuf = 32 * kRowPitch;
+constexpr int kRowBuf = kChunkRows * kRowPitch;
 constexpr int kGradPitch = 36;
 constexpr int kEpiBytes = kEpiWarps * 32 * kGradPitch * 4;
-static_assert(2 * kRowBuf <= kEpiBytes, "epilogue staging");
+static_assert(4 * kRowBuf <= kEpiBytes, "epilogue staging");
 constexpr int kBarBytes = 256;
 constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiBytes + kBarBytes + (2 * (kMaxGroups + 1) + kThreads) * 4;
 static_assert(kSmemBytes <= 232448, "shared memory per CTA");
@@ -68,6 +81,9 @@ struct DenseArgs {
     int inputs, outputs;
     void *out;
     int out_f32, accumulate;
+    int sum_runs;   // kWeightGrad: float32 sums over runs of stages
+    int part_rows;  // kWeightGrad: rows of a group per unit
+    float *parts;   // and where the sums of a group's parts go if it has several
 };
 
 // D f32, A and B bf16, M = 256, N in bits 17-22; A or B M/N-major in bits 15, 16
@@ -82,32 +98,41 @@ __device__ __forceinline__ uint64_t column_major_desc(uint32_t saddr) {
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-__device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
         "%3}], [%4];" ::"r"(dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tma_pair_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
         "%3, %4}], [%5];" ::"r"(dst),
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
+__device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                         uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4, %5}], [%6];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
 
-__device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory"); }
-// The epilogue warps take a tile together or stop together.
-__device__ __forceinline__ bool epi_vote(bool ok) {
+// Barriers 1 and 2: the epilogue's groups of four warps.
+__device__ __forceinline__ void epi_bar(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
+// A group's warps take a tile together or stop together.
+__device__ __forceinline__ bool epi_vote(int group, bool ok) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.and.pred q, 1, %2, p;\n\t"
+        "bar.red.and.pred q, %2, 128, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}\n"
         : "=r"(r)
-        : "r"((uint32_t)ok), "n"(kEpiWarps * 32)
+        : "r"((uint32_t)ok), "r"(1 + group)
         : "memory");
     return r != 0;
 }
@@ -140,21 +165,23 @@ __device__ __forceinline__ void settle() {
     }
 }
 
-// One tile: group, first row of A in its operand (m0), first row of B in the
-// group or first column (n0), columns of the tile (n_valid, and n: the next
-// multiple of 32), stages of the sum.
+// One tile: group, its first row of A in its operand (m0), first row of B in
+// the group or first column (n0), columns of the tile (n_valid, and n: the next
+// multiple of 32), stages of the sum, and the rows row0 .. row0 + rows that it
+// reads (the group's, or a part of them).  part < 0: the unit has all of the
+// group's rows.
 struct Unit {
-    int g, m0, n0, n_valid, n, stages;
+    int g, m0, n0, n_valid, n, stages, row0, rows, part;
 };
 
-// Unit u of the launch.  A group's units run in bands of kBandTiles row tiles
-// (column tiles of the weight gradient): within a band the A tile is the
-// outer index, so that units at work together share operands through L2.
-// Every role walks its units in increasing order.
+// Unit u of the launch.  A group's (a part's) units run in bands of kBandTiles
+// column tiles of D: within a band the A tile is the outer index, so that the
+// units at work together, about 8 x 9 tiles, share operands through L2.  Every
+// role walks its units in increasing order.
 template <GroupedOp OP>
 struct Units {
     const int *start, *tiles;
-    int groups, m_tiles, inputs, outputs;
+    int groups, m_tiles, inputs, outputs, part_rows;
     int g = 0;
     __device__ __forceinline__ int64_t total() const {
         return OP == kWeightGrad ? (int64_t)tiles[groups] : (int64_t)tiles[groups] * m_tiles;
@@ -162,36 +189,46 @@ struct Units {
     __device__ __forceinline__ Unit at(int64_t u) {
         const int64_t per = OP == kWeightGrad ? 1 : m_tiles;
         while (tiles[g + 1] * per <= u) g++;
-        const int64_t r = u - tiles[g] * per;
+        int r = (int)(u - tiles[g] * per);
         Unit w;
         w.g = g;
-        const int rows = start[g + 1] - start[g];
-        int mt, nt;
+        w.row0 = start[g];
+        w.rows = start[g + 1] - start[g];
+        w.part = -1;
+        int n_tiles = tiles[g + 1] - tiles[g];
         if (OP == kWeightGrad) {
-            mt = (int)(r % m_tiles);
-            nt = (int)(r / m_tiles);
-        } else {
-            const int n_tiles = tiles[g + 1] - tiles[g];
-            const int64_t band = r / ((int64_t)kBandTiles * m_tiles);
-            const int first = (int)band * kBandTiles, in_band = min(kBandTiles, n_tiles - first);
-            const int q = (int)(r - band * kBandTiles * m_tiles);
-            mt = q / in_band;
-            nt = first + q % in_band;
+            n_tiles = (inputs + kTileN - 1) / kTileN;
+            if (w.rows > part_rows) {
+                const int area = m_tiles * n_tiles, part = r / area;
+                r -= part * area;
+                w.part = tiles[g] / area + part;
+                w.row0 += part * part_rows;
+                w.rows = min(part_rows, w.rows - part * part_rows);
+            }
         }
-        w.m0 = mt * kTileM;
-        w.n0 = nt * kTileN;
-        w.n_valid = min(kTileN, (OP == kWeightGrad ? inputs : rows) - w.n0);
+        const int band = r / (kBandTiles * m_tiles);
+        const int first = band * kBandTiles, in_band = min(kBandTiles, n_tiles - first);
+        const int q = r - band * kBandTiles * m_tiles;
+        w.m0 = q / in_band * kTileM;
+        w.n0 = (first + q % in_band) * kTileN;
+        w.n_valid = min(kTileN, (OP == kWeightGrad ? inputs : w.rows) - w.n0);
         w.n = (w.n_valid + 31) & ~31;
-        const int sum = OP == kProduct ? inputs : OP == kInputGrad ? outputs : rows;
+        const int sum = OP == kProduct ? inputs : OP == kInputGrad ? outputs : w.rows;
         w.stages = (sum + kStageK - 1) / kStageK;
         return w;
     }
 };
 
+// The tensor maps of a launch.  a, b: the whole boxes (two 64-column chunks of
+// an M- or N-major operand); a_edge, b_edge: one chunk; b_rows: rows of a
+// K-major B in boxes of 32 and 64 rows.
+struct Maps {
+    CUtensorMap a, b, a_edge, b_edge, b_rows[2];
+};
+
 template <GroupedOp OP>
 __global__ void __launch_bounds__(kThreads, 1)
-    grouped_dense_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
-                         const __grid_constant__ CUtensorMap bsmall, const DenseArgs a) {
+    grouped_dense_kernel(const __grid_constant__ Maps maps, const DenseArgs a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *epi = smem + kStages * kStageBytes;
@@ -237,15 +274,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int m_size = OP == kInputGrad ? a.inputs : a.outputs;
     const int m_tiles = (m_size + kTileM - 1) / kTileM;
     const bool counts_ok =
-        group_ranges(a.counts, a.groups, a.rows, OP == kWeightGrad ? 0 : kTileN,
-                     OP == kWeightGrad ? m_tiles * ((a.inputs + kTileN - 1) / kTileN) : 0, start, tiles, scratch);
+        OP == kWeightGrad ? group_ranges(a.counts, a.groups, a.rows, a.part_rows, 1,
+                                         m_tiles * ((a.inputs + kTileN - 1) / kTileN), start, tiles, scratch)
+                          : group_ranges(a.counts, a.groups, a.rows, kTileN, 0, 1, start, tiles, scratch);
     if (!counts_ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_dense_error, 0, kErrBadCounts);
     tc_fence_before();
     __syncthreads();
     cluster_sync();  // the peer's barriers are initialised before any remote operation
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    Units<OP> units{start, tiles, a.groups, m_tiles, a.inputs, a.outputs};
+    Units<OP> units{start, tiles, a.groups, m_tiles, a.inputs, a.outputs, a.part_rows};
     const int64_t total = units.total();
 
     if (warp == 0) {
@@ -257,24 +295,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Unit w = units.at(u);
                 const int half_n = w.n >> 1;  // this CTA's rows (columns) of B
                 const int am = w.m0 + (int)rank * kHalf;
-                const int bn = w.n0 + (int)rank * half_n + (OP == kWeightGrad ? 0 : start[w.g]);
-                const bool small = OP != kWeightGrad && w.n < kTileN;
-                const int boxes = OP == kWeightGrad ? (half_n + 63) / 64 : small ? (half_n + kSmallBox - 1) / kSmallBox : 1;
-                const uint32_t bytes = kOperandBytes + boxes * (OP == kWeightGrad ? kChunkBytes
-                                                                : small           ? kSmallBox * 128
-                                                                                  : kOperandBytes);
-                const int rows_end = start[w.g + 1] - start[w.g];
+                const int bn = w.n0 + (int)rank * half_n + (OP == kWeightGrad ? 0 : w.row0);
+                // an M- or N-major operand's two chunks in one box unless its last column cuts one
+                const int a_cols = OP == kInputGrad ? a.inputs : a.outputs;
+                const bool a_whole = OP == kProduct || am + kHalf <= (a_cols & ~63);
+                const bool b_whole = OP != kWeightGrad || (w.n == kTileN && bn + kHalf <= (a.inputs & ~63));
+                const int b_chunks = OP == kWeightGrad ? (half_n + 63) / 64 : 0;
+                // a K-major B by the smallest box that holds its rows
+                const CUtensorMap *b_map = OP == kWeightGrad || half_n > 64 ? &maps.b : &maps.b_rows[half_n > 32];
+                const uint32_t bytes =
+                    kOperandBytes + (OP == kWeightGrad ? b_chunks * kChunkBytes
+                                     : half_n > 64     ? kOperandBytes
+                                                       : (half_n > 32 ? 64 : 32) * 128);
                 for (int s = 0; s < w.stages; s++, j++) {
                     const int sb = (int)(j % kStages);
                     if (!wait_for(&empty[sb], ((j / kStages) & 1) ^ 1, ab, 1)) {
                         ok = false;
                         break;
                     }
-                    const bool cut = OP == kWeightGrad && (s + 1) * kStageK > rows_end;
+                    const int k0 = s * kStageK;
                     uint32_t bar;
-                    if (cut) {
+                    if (OP == kWeightGrad && k0 + kStageK > w.rows) {
                         mbar_arrive_expect_tx(&tail[sb], bytes);
-                        bar = smem_u32(&tail[sb]);
+                        bar = mapa_shared(smem_u32(&tail[sb]), rank);
                     } else {
                         if (leader) {
                             mbar_arrive_expect_tx(&full[sb], 2 * bytes);
@@ -282,26 +325,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         bar = mapa_shared(smem_u32(&full[sb]), 0);
                     }
-                    if (cut) bar = mapa_shared(bar, rank);
                     const uint32_t sa = smem_u32(smem + sb * kStageBytes), sbb = sa + kOperandBytes;
-                    const int k0 = s * kStageK;
                     if (OP == kProduct) {
-                        tma_pair_3d(sa, &amap, k0, am, w.g, bar);
-                    } else if (OP == kInputGrad) {
-                        tma_pair_3d(sa, &amap, am, k0, w.g, bar);
-                        tma_pair_3d(sa + kChunkBytes, &amap, am + 64, k0, w.g, bar);
+                        tma_pair(sa, &maps.a, k0, am, w.g, bar);
+                    } else if (a_whole) {
+                        if (OP == kInputGrad) tma_pair(sa, &maps.a, 0, k0, am / 64, w.g, bar);
+                        else tma_pair(sa, &maps.a, 0, w.row0 + k0, am / 64, bar);
                     } else {
-                        tma_pair_2d(sa, &amap, am, start[w.g] + k0, bar);
-                        tma_pair_2d(sa + kChunkBytes, &amap, am + 64, start[w.g] + k0, bar);
+                        for (int i = 0; i < 2; i++) {
+                            if (OP == kInputGrad) tma_pair(sa + i * kChunkBytes, &maps.a_edge, am + 64 * i, k0, w.g, bar);
+                            else tma_pair(sa + i * kChunkBytes, &maps.a_edge, am + 64 * i, w.row0 + k0, bar);
+                        }
                     }
-                    if (OP == kWeightGrad) {
-                        for (int i = 0; i < boxes; i++)
-                            tma_pair_2d(sbb + i * kChunkBytes, &bmap, bn + 64 * i, start[w.g] + k0, bar);
-                    } else if (!small) {
-                        tma_pair_2d(sbb, &bmap, k0, bn, bar);
+                    if (OP != kWeightGrad) {
+                        tma_pair(sbb, b_map, k0, bn, bar);
+                    } else if (b_whole) {
+                        tma_pair(sbb, b_map, 0, w.row0 + k0, bn / 64, bar);
                     } else {
-                        for (int i = 0; i < boxes; i++)
-                            tma_pair_2d(sbb + i * kSmallBox * 128, &bsmall, k0, bn + i * kSmallBox, bar);
+                        for (int i = 0; i < b_chunks; i++)
+                            tma_pair(sbb + i * kChunkBytes, &maps.b_edge, bn + 64 * i, w.row0 + k0, bar);
                     }
                 }
             }
@@ -310,111 +352,141 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         // ---------------- MMA issue (leader)
         if (leader && lane == 0) {
-            uint32_t j = 0, tile = 0;
+            uint32_t j = 0, run = 0;  // stages, and accumulators filled
             bool ok = true;
             for (int64_t u = cluster; u < total && ok; u += n_clusters) {
                 const Unit w = units.at(u);
-                if (w.stages == 0) continue;  // no rows: the epilogue writes zeros
-                const uint32_t acc = tile & 1;
-                if (!wait_for(&tmem_empty[acc], ((tile >> 1) & 1) ^ 1, ab, 2)) break;
-                tc_fence_after();
-                const uint32_t d = tmem_base + acc * kTileN, idesc = instr_desc<OP>(w.n);
-                for (int s = 0; s < w.stages; s++, j++) {
-                    const int sb = (int)(j % kStages);
-                    if (!wait_for(&full[sb], (j / kStages) & 1, ab, 3)) {
+                const uint32_t idesc = instr_desc<OP>(w.n);
+                const int run_stages = OP == kWeightGrad && a.sum_runs ? kRunStages : w.stages;
+                for (int s0 = 0; s0 < w.stages && ok; s0 += run_stages, run++) {
+                    const uint32_t acc = run & 1, d = tmem_base + acc * kTileN;
+                    if (!wait_for(&tmem_empty[acc], ((run >> 1) & 1) ^ 1, ab, 2)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + sb * kStageBytes), sbb = sa + kOperandBytes;
-                    const uint64_t ad = OP == kProduct ? sw128_desc(sa) : column_major_desc(sa);
-                    const uint64_t bd = OP == kWeightGrad ? column_major_desc(sbb) : sw128_desc(sbb);
+                    const int s1 = min(w.stages, s0 + run_stages);
+                    for (int s = s0; s < s1; s++, j++) {
+                        const int sb = (int)(j % kStages);
+                        if (!wait_for(&full[sb], (j / kStages) & 1, ab, 3)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t sa = smem_u32(smem + sb * kStageBytes), sbb = sa + kOperandBytes;
+                        const uint64_t ad = OP == kProduct ? sw128_desc(sa) : column_major_desc(sa);
+                        const uint64_t bd = OP == kWeightGrad ? column_major_desc(sbb) : sw128_desc(sbb);
 #pragma unroll
-                    for (int k = 0; k < kStageK / 16; k++)
-                        // 16 terms: 32 bytes of a K-major row, 16 rows of the others
-                        umma2_bf16(d, ad + k * (OP == kProduct ? 2 : 128), bd + k * (OP == kWeightGrad ? 128 : 2), idesc,
-                                   (s | k) != 0);
-                    umma2_commit_mc(&empty[sb], 0x3);
+                        for (int k = 0; k < kStageK / 16; k++)
+                            // 16 terms: 32 bytes of a K-major row, 16 rows of the others
+                            umma2_bf16(d, ad + k * (OP == kProduct ? 2 : 128), bd + k * (OP == kWeightGrad ? 128 : 2),
+                                       idesc, s > s0 || k > 0);
+                        umma2_commit_mc(&empty[sb], 0x3);
+                    }
+                    if (ok) umma2_commit_mc(&tmem_full[acc], 0x3);
                 }
-                if (!ok) break;
-                umma2_commit_mc(&tmem_full[acc], 0x3);
-                tile++;
             }
             if (*ab.own) settle();
         }
     } else if (warp < 2 + kEpiWarps) {
-        // ---------------- epilogue
+        // ---------------- epilogue: this warp has 32 lanes and half the columns of D
         const int quad = warp & 3;  // TMEM lanes 32 * quad ..
-        const int et = threadIdx.x - 64;
+        const int group = (warp - 2) >> 2, et = (threadIdx.x - 64) & 127;
         const uint32_t tmem_empty_leader = mapa_shared(smem_u32(&tmem_empty[0]), 0);
-        uint32_t tile = 0, buf = 0;
+        const uint32_t t_warp = tmem_base + ((uint32_t)(quad * 32) << 16) + group * kHalf;
+        uint32_t run = 0, buf = 0;
+        // the accumulator is in registers: the next tile or run may have it
+        auto release = [&](uint32_t acc) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(tmem_empty_leader + acc * (uint32_t)sizeof(uint64_t));
+        };
         for (int64_t u = cluster; u < total; u += n_clusters) {
             const Unit w = units.at(u);
-            const uint32_t acc = tile & 1;
-            if (w.stages) {
-                const bool ready = wait_for(&tmem_full[acc], (tile >> 1) & 1, ab, 4);
-                if (!epi_vote(ready)) break;
-                tc_fence_after();
-            }
-            const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * kTileN;
-            const int chunks = (w.n_valid + 31) / 32;
             const int m_first = w.m0 + (int)rank * kHalf;
-            for (int c = 0; c < chunks; c++) {
-                uint32_t v[32];
-                if (w.stages) {
-                    tmem_ld16(t_row + c * 32, *reinterpret_cast<uint32_t(*)[16]>(v));
-                    tmem_ld16(t_row + c * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
-                    tmem_ld_wait();
-                    if (c == chunks - 1) {
-                        // the accumulator is in registers: the next tile may have it
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_remote(tmem_empty_leader + acc * (uint32_t)sizeof(uint64_t));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = 0;
-                }
-                if (OP != kWeightGrad) {
+            const int left = w.n_valid - group * kHalf;  // columns for this group
+            if (OP != kWeightGrad) {
+                const uint32_t acc = run & 1;
+                const bool ready = wait_for(&tmem_full[acc], (run >> 1) & 1, ab, 4);
+                if (!epi_vote(group, ready)) break;
+                tc_fence_after();
+                run++;
+                const int chunks = left <= 0 ? 0 : left >= kHalf ? kHalf / kChunkRows : (left + kChunkRows - 1) / kChunkRows;
+                if (chunks == 0) release(acc);
+                for (int c = 0; c < chunks; c++) {
                     // lanes are output features, v[i] row i of the chunk
-                    uint8_t *stage = epi + buf * kRowBuf;
+                    uint32_t v[kChunkRows];
+                    tmem_ld16(t_warp + acc * kTileN + c * kChunkRows, v);
+                    tmem_ld_wait();
+                    if (c == chunks - 1) release(acc);
+                    uint8_t *stage = epi + (group * 2 + buf) * kRowBuf;
                     __nv_bfloat16 *col = reinterpret_cast<__nv_bfloat16 *>(stage) + quad * 32 + lane;
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
+                    for (int i = 0; i < kChunkRows; i++)
                         col[i * (kRowPitch / 2)] = __float2bfloat16(__uint_as_float(v[i]));
-                    epi_bar();
-                    const int64_t row0 = (int64_t)start[w.g] + w.n0 + c * 32;
+                    epi_bar(group);
+                    const int first = c * kChunkRows;
+                    const int64_t row0 = (int64_t)w.row0 + w.n0 + group * kHalf + first;
                     __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + row0 * m_size + m_first;
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
+                    for (int q = 0; q < kChunkRows / 8; q++) {
                         const int r = q * 8 + (et >> 4), seg = et & 15;
-                        if (c * 32 + r < w.n_valid && m_first + seg * 8 < m_size)
+                        if (first + r < left && m_first + seg * 8 < m_size)
                             *reinterpret_cast<uint4 *>(out + (int64_t)r * m_size + seg * 8) =
                                 *reinterpret_cast<const uint4 *>(stage + r * kRowPitch + seg * 16);
                     }
                     buf ^= 1;  // the next chunk's barrier separates this buffer's reads from its next writes
-                } else {
-                    // lanes are rows of dW, v[i] column i of the chunk
-                    float *stage = reinterpret_cast<float *>(epi) + quad * 32 * kGradPitch;
+                }
+            } else {
+                // lanes are rows of dW; the runs' sums in registers
+                const int run_stages = a.sum_runs ? kRunStages : w.stages;
+                float sum[kHalf];
+#pragma unroll
+                for (int i = 0; i < kHalf; i++) sum[i] = 0.f;
+                bool ok = true;
+                for (int s0 = 0; s0 < w.stages; s0 += run_stages, run++) {
+                    const uint32_t acc = run & 1;
+                    const bool ready = wait_for(&tmem_full[acc], (run >> 1) & 1, ab, 4);
+                    if (!(ok = epi_vote(group, ready))) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < kHalf / 16; c++)
+                        if (c * 16 < left) {
+                            uint32_t v[16];
+                            tmem_ld16(t_warp + acc * kTileN + c * 16, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; i++) sum[c * 16 + i] += __uint_as_float(v[i]);
+                        }
+                    release(acc);
+                }
+                if (!ok) break;
+                float *stage = reinterpret_cast<float *>(epi) + (warp - 2) * 32 * kGradPitch;
+                const bool f32 = a.out_f32 || w.part >= 0, add = a.accumulate && w.part < 0;
+                void *base = w.part >= 0 ? (void *)a.parts : a.out;
+                const int64_t o0 = ((int64_t)(w.part >= 0 ? w.part : w.g) * a.outputs + m_first + quad * 32) * a.inputs +
+                                   w.n0 + group * kHalf;
+                const int rows = a.outputs - m_first - quad * 32;  // of dW for this warp
+#pragma unroll
+                for (int c = 0; c < kHalf / 32; c++) {
+                    if (c * 32 >= left) break;
                     float4 *mine = reinterpret_cast<float4 *>(stage + lane * kGradPitch);
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        mine[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
-                                              __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+                        mine[i] = make_float4(sum[c * 32 + 4 * i], sum[c * 32 + 4 * i + 1], sum[c * 32 + 4 * i + 2],
+                                              sum[c * 32 + 4 * i + 3]);
                     __syncwarp();
-                    const int col0 = w.n0 + c * 32;
-                    const int64_t o0 = ((int64_t)w.g * a.outputs + m_first + quad * 32) * a.inputs + col0;
-                    if (a.out_f32) {
-                        float *out = (float *)a.out + o0;
+                    if (f32) {
                         const int cc = (lane & 7) * 4;
+                        float *out = (float *)base + o0 + c * 32 + cc;
 #pragma unroll
                         for (int q = 0; q < 8; q++) {
                             const int r = q * 4 + (lane >> 3);
-                            if (m_first + quad * 32 + r < a.outputs && col0 + cc < a.inputs) {
-                                float4 *p = reinterpret_cast<float4 *>(out + (int64_t)r * a.inputs + cc);
+                            if (r < rows && c * 32 + cc < left) {
+                                float4 *p = reinterpret_cast<float4 *>(out + (int64_t)r * a.inputs);
                                 float4 x = *reinterpret_cast<const float4 *>(stage + r * kGradPitch + cc);
-                                if (a.accumulate) {
+                                if (add) {
                                     const float4 b = *p;
                                     x.x += b.x, x.y += b.y, x.z += b.z, x.w += b.w;
                                 }
@@ -422,28 +494,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     } else {
-                        __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + o0;
+                        using Io = VecIO<__nv_bfloat16, float, 8>;
                         const int cc = (lane & 3) * 8;
+                        __nv_bfloat16 *out = (__nv_bfloat16 *)base + o0 + c * 32 + cc;
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
                             const int r = q * 8 + (lane >> 2);
-                            if (m_first + quad * 32 + r < a.outputs && col0 + cc < a.inputs) {
-                                __nv_bfloat16 *p = out + (int64_t)r * a.inputs + cc;
+                            if (r < rows && c * 32 + cc < left) {
+                                __nv_bfloat16 *p = out + (int64_t)r * a.inputs;
                                 float x[8], b[8];
 #pragma unroll
                                 for (int i = 0; i < 8; i++) x[i] = stage[r * kGradPitch + cc + i];
-                                if (a.accumulate) {
-                                    VecIO<__nv_bfloat16, float, 8>::unpack(VecIO<__nv_bfloat16, float, 8>::load(p), b);
+                                if (add) {
+                                    Io::unpack(Io::load(p), b);
 #pragma unroll
                                     for (int i = 0; i < 8; i++) x[i] += b[i];
                                 }
-                                VecIO<__nv_bfloat16, float, 8>::store(p, x);
+                                Io::store(p, x);
                             }
                         }
                     }
                 }
             }
-            if (w.stages) tile++;
         }
     } else if (OP == kWeightGrad) {
         // ---------------- rows past a group's end, in the sum's last stage, become zeros
@@ -451,8 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int64_t u = cluster; u < total && ok; u += n_clusters) {
             const Unit w = units.at(u);
-            const int rows = start[w.g + 1] - start[w.g];
-            const int valid = rows % kStageK;
+            const int valid = w.rows % kStageK;
             j += w.stages;
             if (w.stages == 0 || valid == 0) continue;
             const int sb = (int)((j - 1) % kStages);
@@ -483,25 +554,84 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// A bf16 view with `dims` (innermost first; each further one dense) and the
-// given box, 128-byte swizzle; what lies outside reads as zeros.
-int encode_view(CUtensorMap *map, const void *base, int n_dims, const int64_t *size, const int *box) {
+// A bf16 view of `base` with 128-byte swizzle: axis i has size[i] elements
+// stride[i] elements apart (axis 0 one) and box[i] of them per box; what lies
+// outside the sizes reads as zeros.
+struct View {
+    int axes;
+    int64_t size[4], stride[4];
+    int box[4];
+};
+int encode_view(CUtensorMap *map, const void *base, const View &v) {
     auto enc = tensor_map_encoder();
     if (!enc) return fail(GTMOE_ECUDA, "cuTensorMapEncodeTiled is not available");
-    cuuint64_t dims[3], strides[2];
-    cuuint32_t boxes[3], ones[3] = {1, 1, 1};
-    cuuint64_t bytes = 2;
-    for (int i = 0; i < n_dims; i++) {
-        dims[i] = (cuuint64_t)size[i];
-        boxes[i] = (cuuint32_t)box[i];
-        if (i) strides[i - 1] = bytes;
-        bytes *= dims[i];
+    cuuint64_t dims[4], strides[3];
+    cuuint32_t boxes[4], ones[4] = {1, 1, 1, 1};
+    for (int i = 0; i < v.axes; i++) {
+        dims[i] = (cuuint64_t)v.size[i];
+        boxes[i] = (cuuint32_t)v.box[i];
+        if (i) strides[i - 1] = (cuuint64_t)v.stride[i] * 2;
     }
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)n_dims, const_cast<void *>(base), dims,
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)v.axes, const_cast<void *>(base), dims,
                            strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(GTMOE_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return 0;
+}
+// rows x columns, `cols` per row, in boxes of box_rows rows x 64 columns
+View matrix(int64_t rows, int64_t cols, int box_rows) { return {2, {cols, rows}, {1, cols}, {64, box_rows}}; }
+// the same as chunks of 64 columns, two to a box; only whole chunks
+View chunks(int64_t rows, int64_t cols) {
+    return {3, {64, rows, cols / 64 ? cols / 64 : 1}, {1, cols, 64}, {64, kStageK, 2}};
+}
+
+// Rows of a group per unit of the weight gradient.  With tiles for every CTA
+// pair a unit has all of a group's rows; with fewer the groups are split, into
+// about two units per pair, and the parts' sums added by a second kernel
+// (1 group of 65536 rows, 512 x 512: 467 us unsplit).  Short groups are not:
+// their units end before the second kernel would.
+int part_rows(int64_t rows, int64_t inputs, int64_t outputs, int groups) {
+    const int64_t area = ((outputs + kTileM - 1) / kTileM) * ((inputs + kTileN - 1) / kTileN);
+    if (area * groups >= 74 || rows < (int64_t)groups * 2048) return kAnyRows;
+    const int64_t run = kRunStages * kStageK, want = (rows * area / 148 + run - 1) / run * run;
+    return (int)(want < run ? run : want);
+}
+
+// Adds the parts' sums of every group that was split, in order, four values
+// per thread.
+__global__ void __launch_bounds__(256) add_parts_kernel(const DenseArgs a) {
+    __shared__ int start[kMaxGroups + 1], first[kMaxGroups + 1], scratch[256];
+    group_ranges(a.counts, a.groups, a.rows, a.part_rows, 1, 1, start, first, scratch);
+    const int64_t area = (int64_t)a.outputs * a.inputs;
+    for (int g = 0; g < a.groups; g++) {
+        const int parts = first[g + 1] - first[g];
+        if (parts < 2) continue;
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < area; i += (int64_t)gridDim.x * 1024) {
+            const float *p = a.parts + first[g] * area + i;
+            float4 s = *reinterpret_cast<const float4 *>(p);
+            for (int q = 1; q < parts; q++) {
+                const float4 v = *reinterpret_cast<const float4 *>(p + q * area);
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            const int64_t o = g * area + i;
+            if (a.out_f32) {
+                float4 *out = reinterpret_cast<float4 *>((float *)a.out + o);
+                if (a.accumulate) {
+                    const float4 b = *out;
+                    s.x += b.x, s.y += b.y, s.z += b.z, s.w += b.w;
+                }
+                *out = s;
+            } else {
+                __nv_bfloat162 *out = reinterpret_cast<__nv_bfloat162 *>((__nv_bfloat16 *)a.out + o);
+                if (a.accumulate) {
+                    const float2 b0 = __bfloat1622float2(out[0]), b1 = __bfloat1622float2(out[1]);
+                    s.x += b0.x, s.y += b0.y, s.z += b1.x, s.w += b1.y;
+                }
+                out[0] = __floats2bfloat162_rn(s.x, s.y);
+                out[1] = __floats2bfloat162_rn(s.z, s.w);
+            }
+        }
+    }
 }
 
 template <GroupedOp OP>
@@ -530,22 +660,28 @@ int launch(const GroupedProduct &p, int device, cudaStream_t st) {
         if (pairs < 1) return fail(GTMOE_ECUDA, "no CTA pair of the grouped product fits on this device");
         if (device < 64) resident[device].store(pairs);
     }
-    CUtensorMap amap, bmap, bsmall;
-    const int64_t wdims[3] = {p.inputs, p.outputs, p.groups}, xdims[2] = {p.inputs, p.rows}, ydims[2] = {p.outputs, p.rows};
-    const int rows_box[2] = {kStageK, kHalf}, small_box[2] = {kStageK, kSmallBox}, sum_box[2] = {64, kStageK};
-    const int w_box[3] = {kStageK, kHalf, 1}, wt_box[3] = {64, kStageK, 1};
-    if (OP == kProduct) {
-        GT_CHECK(encode_view(&amap, p.b, 3, wdims, w_box));
-        GT_CHECK(encode_view(&bmap, p.a, 2, xdims, rows_box));
-        GT_CHECK(encode_view(&bsmall, p.a, 2, xdims, small_box));
-    } else if (OP == kInputGrad) {
-        GT_CHECK(encode_view(&amap, p.b, 3, wdims, wt_box));
-        GT_CHECK(encode_view(&bmap, p.a, 2, ydims, rows_box));
-        GT_CHECK(encode_view(&bsmall, p.a, 2, ydims, small_box));
+    Maps m;
+    const int64_t in = p.inputs, out = p.outputs, rows = p.rows;
+    if (OP == kWeightGrad) {
+        GT_CHECK(encode_view(&m.a, p.a, chunks(rows, out)));
+        GT_CHECK(encode_view(&m.a_edge, p.a, matrix(rows, out, kStageK)));
+        GT_CHECK(encode_view(&m.b, p.b, chunks(rows, in)));
+        GT_CHECK(encode_view(&m.b_edge, p.b, matrix(rows, in, kStageK)));
+        m.b_rows[0] = m.b_rows[1] = m.b_edge;
     } else {
-        GT_CHECK(encode_view(&amap, p.a, 2, ydims, sum_box));
-        GT_CHECK(encode_view(&bmap, p.b, 2, xdims, sum_box));
-        bsmall = bmap;
+        const int64_t sum = OP == kProduct ? in : out, group = in * out;
+        if (OP == kProduct) {
+            GT_CHECK(encode_view(&m.a, p.b, {3, {in, out, p.groups}, {1, in, group}, {kStageK, kHalf, 1}}));
+            m.a_edge = m.a;
+        } else {
+            GT_CHECK(encode_view(&m.a, p.b,
+                                 {4, {64, out, in / 64 ? in / 64 : 1, p.groups}, {1, in, 64, group}, {64, kStageK, 2, 1}}));
+            GT_CHECK(encode_view(&m.a_edge, p.b, {3, {in, out, p.groups}, {1, in, group}, {64, kStageK, 1}}));
+        }
+        GT_CHECK(encode_view(&m.b, p.a, matrix(rows, sum, kHalf)));
+        GT_CHECK(encode_view(&m.b_rows[0], p.a, matrix(rows, sum, 32)));
+        GT_CHECK(encode_view(&m.b_rows[1], p.a, matrix(rows, sum, 64)));
+        m.b_edge = m.b;
     }
     DenseArgs a;
     a.counts = p.counts;
@@ -556,14 +692,24 @@ int launch(const GroupedProduct &p, int device, cudaStream_t st) {
     a.out = p.c;
     a.out_f32 = p.out_dtype == GTMOE_DTYPE_F32;
     a.accumulate = p.accumulate;
-    // at most this many tiles: the rows of a group end inside a tile
-    const int64_t m_tiles = ((OP == kInputGrad ? p.inputs : p.outputs) + kTileM - 1) / kTileM;
-    const int64_t n_tiles = OP == kWeightGrad ? p.groups * ((p.inputs + kTileN - 1) / kTileN)
-                                              : p.rows / kTileN + (p.rows < p.groups ? p.rows : p.groups);
+    a.part_rows = OP == kWeightGrad ? part_rows(rows, in, out, p.groups) : kAnyRows;
+    a.parts = (float *)p.workspace;
+    a.sum_runs = a.out_f32 || a.part_rows != kAnyRows;
+    // at most this many tiles: the rows of a group end inside a tile or part
+    const int64_t m_tiles = ((OP == kInputGrad ? in : out) + kTileM - 1) / kTileM;
+    const int64_t some = rows < p.groups ? rows : p.groups;
+    const int64_t n_tiles = OP == kWeightGrad ? (p.groups + rows / a.part_rows) * ((in + kTileN - 1) / kTileN)
+                                              : rows / kTileN + some;
     const int64_t most = m_tiles * n_tiles;
     cfg.gridDim = dim3(2 * (unsigned)(most < pairs ? most : pairs));
-    GT_CUDA(cudaLaunchKernelEx(&cfg, kern, amap, bmap, bsmall, a));
+    GT_CUDA(cudaLaunchKernelEx(&cfg, kern, m, a));
     note_launches(1);
+    if (OP == kWeightGrad && a.part_rows != kAnyRows) {
+        const int64_t blocks = (in * out / 4 + 255) / 256;
+        add_parts_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(a);
+        GT_CUDA(cudaGetLastError());
+        note_launches(1);
+    }
     return 0;
 }
 
@@ -581,6 +727,11 @@ int launch_grouped_dense(const GroupedProduct &p, int device, cudaStream_t st) {
     if (p.op == kProduct) return launch<kProduct>(p, device, st);
     if (p.op == kInputGrad) return launch<kInputGrad>(p, device, st);
     return launch<kWeightGrad>(p, device, st);
+}
+
+int64_t grouped_dense_workspace(int64_t rows, int64_t inputs, int64_t outputs, int groups) {
+    const int64_t part = part_rows(rows, inputs, outputs, groups);
+    return part == kAnyRows ? 0 : (rows / part + groups) * inputs * outputs * 4;
 }
 
 int grouped_dense_take_error(int *code) {

@@ -24,8 +24,9 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
     __shared__ int start[kMaxGroups + 1], tiles[kMaxGroups + 1], scratch[kThreads];
     const int64_t n_j = OP == kProduct ? a.outputs : a.inputs;
     const int64_t j_tiles = (n_j + kTile - 1) / kTile;
-    const bool ok = group_ranges(a.counts, a.groups, a.rows, OP == kWeightGrad ? 0 : kTile,
-                                 (int)((a.outputs + kTile - 1) / kTile), start, tiles, scratch);
+    const bool ok = OP == kWeightGrad ? group_ranges(a.counts, a.groups, a.rows, kAnyRows, 1,
+                                                     (int)((a.outputs + kTile - 1) / kTile), start, tiles, scratch)
+                                      : group_ranges(a.counts, a.groups, a.rows, kTile, 0, 1, start, tiles, scratch);
     if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_error, 0, kErrBadCounts);
     const int64_t total = (int64_t)tiles[a.groups] * j_tiles;
     const T *A = (const T *)a.a, *B = (const T *)a.b;
@@ -111,7 +112,7 @@ int launch_simt_op(const GroupedProduct &p, cudaStream_t st) {
     return launch_simt<T, ACC, float, kWeightGrad>(p, st);
 }
 
-int run_grouped(const GroupedProduct &p, const char *a_name, const char *b_name, const char *c_name, void *stream) {
+int check_sizes(const GroupedProduct &p) {
     if (!known_dtype(p.dtype) || !known_dtype(p.out_dtype)) return fail(GTMOE_EINVAL, "grouped product: unknown dtype");
     if (p.out_dtype != p.dtype && !(p.dtype == GTMOE_DTYPE_BF16 && p.out_dtype == GTMOE_DTYPE_F32))
         return fail(GTMOE_EINVAL, "grouped product: weight gradients have the operands' dtype, or float32 beside bfloat16");
@@ -126,6 +127,12 @@ int run_grouped(const GroupedProduct &p, const char *a_name, const char *b_name,
         return fail(GTMOE_EINVAL, "grouped product: an operand is too large");
     if ((p.outputs + kTile - 1) / kTile * p.groups > 0x7fffffff)
         return fail(GTMOE_EINVAL, "grouped product: too many outputs for %d groups", p.groups);
+    return 0;
+}
+
+int run_grouped(const GroupedProduct &p, const char *a_name, const char *b_name, const char *c_name,
+                int64_t workspace_bytes, void *stream) {
+    GT_CHECK(check_sizes(p));
     if (p.rows == 0 && p.op != kWeightGrad) return 0;
     if (p.rows == 0 && p.accumulate) return 0;
     if ((p.rows > 0 && (!p.a || !p.b)) || !p.c || !p.counts)
@@ -139,9 +146,19 @@ int run_grouped(const GroupedProduct &p, const char *a_name, const char *b_name,
                                             : wn * (int64_t)dtype_size(p.out_dtype);
     if (ranges_overlap(p.c, cb, p.a, ab) || ranges_overlap(p.c, cb, p.b, bb) || ranges_overlap(p.c, cb, p.counts, 8 * (int64_t)p.groups))
         return fail(GTMOE_EINVAL, "grouped product: %s overlaps another argument", c_name);
+    const int64_t need = p.op == kWeightGrad && grouped_dense_usable(p)
+                             ? grouped_dense_workspace(p.rows, p.inputs, p.outputs, p.groups)
+                             : 0;
+    if (need && (!p.workspace || workspace_bytes < need))
+        return fail(GTMOE_EINVAL, "grouped product: the weight gradients need %lld bytes of workspace, got %lld",
+                    (long long)need, (long long)(p.workspace ? workspace_bytes : 0));
+    if (ranges_overlap(p.workspace, need, p.a, ab) || ranges_overlap(p.workspace, need, p.b, bb) ||
+        ranges_overlap(p.workspace, need, p.c, cb) || ranges_overlap(p.workspace, need, p.counts, 8 * (int64_t)p.groups))
+        return fail(GTMOE_EINVAL, "grouped product: workspace overlaps another argument");
     DeviceScope scope;
     GT_CHECK(scope.enter({{p.c, c_name, dtype_size(p.out_dtype)}, {ab ? p.a : nullptr, a_name, (size_t)es},
-                          {bb ? p.b : nullptr, b_name, (size_t)es}, {p.counts, "counts", 8}}));
+                          {bb ? p.b : nullptr, b_name, (size_t)es}, {p.counts, "counts", 8},
+                          {need ? p.workspace : nullptr, "workspace", 16}}));
     cudaStream_t st = (cudaStream_t)stream;
     if (grouped_dense_usable(p)) return launch_grouped_dense(p, scope.device(), st);
     if (p.dtype == GTMOE_DTYPE_F64) return launch_simt_op<double, double>(p, st);
@@ -171,21 +188,32 @@ extern "C" {
 
 int gtmoe_grouped_product(const void *x, const void *w, int dtype, int64_t rows, int64_t inputs, int64_t outputs,
                           int groups, const int64_t *counts, void *y, void *stream) {
-    const GroupedProduct p = {kProduct, dtype, dtype, 0, rows, inputs, outputs, groups, counts, x, w, y};
-    return run_grouped(p, "x", "w", "y", stream);
+    const GroupedProduct p = {kProduct, dtype, dtype, 0, rows, inputs, outputs, groups, counts, x, w, y, nullptr};
+    return run_grouped(p, "x", "w", "y", 0, stream);
 }
 
 int gtmoe_grouped_product_input_grad(const void *dy, const void *w, int dtype, int64_t rows, int64_t inputs,
                                      int64_t outputs, int groups, const int64_t *counts, void *dx, void *stream) {
-    const GroupedProduct p = {kInputGrad, dtype, dtype, 0, rows, inputs, outputs, groups, counts, dy, w, dx};
-    return run_grouped(p, "dy", "w", "dx", stream);
+    const GroupedProduct p = {kInputGrad, dtype, dtype, 0, rows, inputs, outputs, groups, counts, dy, w, dx, nullptr};
+    return run_grouped(p, "dy", "w", "dx", 0, stream);
+}
+
+int gtmoe_grouped_product_workspace(int dtype, int64_t rows, int64_t inputs, int64_t outputs, int groups,
+                                    int64_t *bytes) {
+    const GroupedProduct p = {kWeightGrad, dtype, dtype, 0, rows, inputs, outputs, groups, nullptr, nullptr, nullptr, nullptr, nullptr};
+    GT_CHECK(check_sizes(p));
+    if (!bytes) return fail(GTMOE_EINVAL, "grouped product: bytes is NULL");
+    // whether the operands' addresses suit the tensor cores is not known here
+    *bytes = grouped_dense_usable(p) ? grouped_dense_workspace(rows, inputs, outputs, groups) : 0;
+    return 0;
 }
 
 int gtmoe_grouped_product_weight_grad(const void *dy, const void *x, int dtype, int64_t rows, int64_t inputs,
                                       int64_t outputs, int groups, const int64_t *counts, void *dw, int dw_dtype,
-                                      int accumulate, void *stream) {
-    const GroupedProduct p = {kWeightGrad, dtype, dw_dtype, accumulate, rows, inputs, outputs, groups, counts, dy, x, dw};
-    return run_grouped(p, "dy", "x", "dw", stream);
+                                      int accumulate, void *workspace, int64_t workspace_bytes, void *stream) {
+    const GroupedProduct p = {kWeightGrad, dtype, dw_dtype, accumulate, rows, inputs, outputs,
+                              groups,      counts, dy,      x,          dw,   workspace};
+    return run_grouped(p, "dy", "x", "dw", workspace_bytes, stream);
 }
 
 }  // extern "C"

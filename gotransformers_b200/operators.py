@@ -238,8 +238,15 @@ def grouped_product_weight_gradients(output_gradients, x, counts, weight_grad=No
     elif dtype is not None and weight_grad.dtype != dtype:
         raise ValueError(f"weight_grad is {weight_grad.dtype} but dtype {dtype}")
     pdw = _tensor("weight_grad", weight_grad, (groups, outputs, inputs), None, g)
+    nbytes, work = ctypes.c_int64(0), None
+    check(_lib.lib().gtmoe_grouped_product_workspace(_code(g.dtype), rows, inputs, outputs, groups,
+                                                     ctypes.byref(nbytes)))
+    if nbytes.value:
+        work = torch.empty(nbytes.value, dtype=torch.uint8, device=g.device)
     check(_lib.lib().gtmoe_grouped_product_weight_grad(pg, px, _code(g.dtype), rows, inputs, outputs, groups, pc, pdw,
-                                                       _code(weight_grad.dtype), int(accumulate), _stream(g)))
+                                                       _code(weight_grad.dtype), int(accumulate),
+                                                       work.data_ptr() if work is not None else None, nbytes.value,
+                                                       _stream(g)))
     return weight_grad
 
 

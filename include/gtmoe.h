@@ -373,14 +373,18 @@ GTMOE_API int gtmoe_set_dropout(gtmoe_t h, double rate, uint64_t seed, uint64_t 
  * written.  A negative count (taken as 0) or a sum above `rows` (rows past the
  * end left out) is reported by gtmoe_operators_check.  No output may be an
  * input.  bfloat16 operands with inputs and outputs a multiple of 8 that
- * start on 16 bytes run on the tensor cores. */
+ * start on 16 bytes run on the tensor cores.  The weight gradient takes the
+ * workspace that gtmoe_grouped_product_workspace names (often none). */
 GTMOE_API int gtmoe_grouped_product(const void *x, const void *w, int dtype, int64_t rows, int64_t inputs,
                           int64_t outputs, int groups, const int64_t *counts, void *y, void *stream);
 GTMOE_API int gtmoe_grouped_product_input_grad(const void *dy, const void *w, int dtype, int64_t rows, int64_t inputs,
                                      int64_t outputs, int groups, const int64_t *counts, void *dx, void *stream);
+GTMOE_API int gtmoe_grouped_product_workspace(int dtype, int64_t rows, int64_t inputs, int64_t outputs, int groups,
+                                    int64_t *bytes);
 GTMOE_API int gtmoe_grouped_product_weight_grad(const void *dy, const void *x, int dtype, int64_t rows,
                                       int64_t inputs, int64_t outputs, int groups, const int64_t *counts, void *dw,
-                                      int dw_dtype, int accumulate, void *stream);
+                                      int dw_dtype, int accumulate, void *workspace, int64_t workspace_bytes,
+                                      void *stream);
 
 /* What the grouped products' kernels recorded on `device` since the last
  * check: waits for the device, then 0, GTMOE_EINVAL (refused counts) or

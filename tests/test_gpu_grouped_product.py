@@ -99,6 +99,34 @@ def test_long_sums():
     check_exact([20, 300], 264, 4104, BF16, F32)
 
 
+@pytest.mark.parametrize("counts", [[5000], [3000, 5001], [0, 9000, 1, 0], [2049, 512, 4096, 7000], [16384]], ids=str)
+@pytest.mark.parametrize("inputs,outputs", [(256, 256), (72, 264), (520, 40)])
+def test_weight_gradients_whose_sums_are_split(counts, inputs, outputs):
+    """Few tiles and many rows: parts of a group in units of their own, added by a second kernel."""
+    assert outputs * inputs <= 1 << 17
+    check_exact(counts, inputs, outputs, BF16, F32)
+    check_exact(counts, inputs, outputs, BF16, BF16)
+    x, _, dy = make(counts, inputs, outputs, BF16, 3, whole=True)
+    ref = R.grouped_weight_gradients(dy, x, counts)
+    for dtype in (F32, BF16):
+        before = torch.randint(-9, 10, ref.shape).to(dtype)
+        dw = before.cuda()
+        moe.grouped_product_weight_gradients(dy.cuda(), x.cuda(), device_counts(counts), weight_grad=dw)
+        assert torch.equal(dw.cpu(), (ref + before.double()).to(dtype))
+
+
+@pytest.mark.parametrize("rows,groups", [(1536, 1), (65536, 1), (20000, 3), (40000, 80)])
+def test_float32_weight_gradients_keep_their_digits(rows, groups):
+    """Runs of 512 rows are 32 additions that cut at most 2^-23 of the sum
+    each; the runs (at most 128) are added with rounding.  Relative to the sums
+    themselves, which random terms bring to about the same size as any part's:
+    32 * 2^-23 + 128 * 2^-24.  One run over 65536 rows would lose 6.6e-5."""
+    counts = [rows // groups] * groups
+    x, _, dy = make(counts, 64, 72, BF16, 17)
+    dw = moe.grouped_product_weight_gradients(dy.cuda(), x.cuda(), device_counts(counts), dtype=F32)
+    R.near("dw", dw, R.grouped_weight_gradients(dy, x, counts), 32 * 2.0**-23 + 128 * 2.0**-24)
+
+
 def test_many_groups():
     g = torch.Generator().manual_seed(8)
     counts = torch.randint(0, 6, (1024,), generator=g).tolist()

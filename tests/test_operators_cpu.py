@@ -55,11 +55,11 @@ def product(**kw):
 
 def weight_grad(**kw):
     dy, x, c, dw = addresses(4)
-    a = dict(dy=dy, x=x, dtype=2, rows=16, inputs=8, outputs=8, groups=2, counts=c, dw=dw, wdtype=2, acc=0)
+    a = dict(dy=dy, x=x, dtype=2, rows=16, inputs=8, outputs=8, groups=2, counts=c, dw=dw, wdtype=2, acc=0, work=None, bytes=0)
     a.update(kw)
     return _lib.lib().gtmoe_grouped_product_weight_grad(a["dy"], a["x"], a["dtype"], a["rows"], a["inputs"],
                                                         a["outputs"], a["groups"], a["counts"], a["dw"], a["wdtype"],
-                                                        a["acc"], None)
+                                                        a["acc"], a["work"], a["bytes"], None)
 
 
 @pytest.mark.parametrize("call", [norm_forward, norm_backward, drop, product, weight_grad])
@@ -126,6 +126,11 @@ def test_good_arguments_reach_the_device_check(call):
     (weight_grad, dict(dtype=1, wdtype=2)),
     (weight_grad, dict(dw=A + STEP)),
     (weight_grad, dict(dw=None)),
+    # one group of many rows and few outputs: its sums are split, into workspace
+    (weight_grad, dict(groups=1, rows=1 << 16)),
+    (weight_grad, dict(groups=1, rows=1 << 16, work=A + 4 * STEP, bytes=64)),
+    (weight_grad, dict(groups=1, rows=1 << 16, work=A, bytes=1 << 27)),
+    (weight_grad, dict(groups=1, rows=1 << 16, work=A + 4 * STEP + 4, bytes=1 << 27)),
 ])
 def test_refusals(call, bad):
     assert call(**bad) == EINVAL
@@ -146,6 +151,12 @@ def test_workspace_size():
     assert 0 < n.value <= 1000 * 64 * 8
     assert _lib.lib().gtmoe_layer_norm_workspace(2, -1, 64, ctypes.byref(n)) == EINVAL
     assert _lib.lib().gtmoe_layer_norm_workspace(2, 1, 64, None) == EINVAL
+    f = _lib.lib().gtmoe_grouped_product_workspace
+    assert f(2, 1 << 16, 256, 256, 1, ctypes.byref(n)) == 0 and 0 < n.value <= 1 << 27
+    assert f(2, 1 << 16, 2048, 2048, 64, ctypes.byref(n)) == 0 and n.value == 0  # tiles for every CTA pair
+    assert f(1, 1 << 16, 256, 256, 1, ctypes.byref(n)) == 0 and n.value == 0  # float32
+    assert f(2, 1 << 16, 256, 256, 0, ctypes.byref(n)) == EINVAL
+    assert f(2, 1 << 16, 256, 256, 1, None) == EINVAL
 
 
 def test_set_dropout_refuses_without_a_handle():
