@@ -17,11 +17,12 @@
 // SBO = 8 rows of the sum).
 //
 // Each CTA stages its 128 rows of A and its half of B in shared memory by TMA
-// (64 terms of the sum per stage, 128-byte swizzle), one TMA instruction per
-// operand: a CTA issues one per about 200 clocks whatever its size, so that a
-// stage of four 8 KB boxes took 826 clocks where the MMAs need 512.  An M- or
-// N-major operand is therefore viewed as 64-column chunks x rows, two chunks to
-// a box, except where a chunk is cut by the operand's last column.  Terms past
+// (64 terms of the sum per stage, 128-byte swizzle), each operand by a warp of
+// its own and in one TMA instruction: a thread issues one per about 200 clocks
+// whatever its size, so that a stage of four 8 KB boxes from one thread took
+// 826 clocks where the MMAs need 512.  An M- or N-major operand is therefore
+// viewed as 64-column chunks x rows, two chunks to a box, except where a chunk
+// is cut by the operand's last column.  Terms past
 // the end of the sum's axis are read as zeros by TMA, from a view of the
 // weights with an axis for the groups, so that the next group's weights are
 // never multiplied.  The sum over rows ends inside a stage: there a warp of
@@ -30,15 +31,15 @@
 //
 // The tensor cores cut every addition to an accumulator towards zero: over n
 // rows the sums shrink by about n / 16 * 2^-24.2 (measured: 4.0e-7 at 512 rows,
-// 6.6e-5 at 65536), far more than float32 rounding.  The weight gradient,
+// 6.6e-5 at 65536 rows), far more than float32 rounding.  The weight gradient,
 // whose result may be float32 and whose sums are the long ones, is therefore
 // accumulated in runs of kRunStages stages; the epilogue adds the runs in
 // registers, with rounding, while the next run is multiplied.  Results in bf16
 // keep one sum: their rounding is 2^-9.
 //
-// Persistent kernel, one CTA per SM; warp 0 TMA, warp 1 MMA issue (leader),
-// warps 2-9 epilogue (TMEM -> bf16 / float32 -> shared memory -> coalesced
-// rows), warp 10 zeroes row tails.  Two accumulators: the epilogue of a tile
+// Persistent kernel, one CTA per SM; warp 0 loads A, warp 1 issues the MMAs
+// (leader), warps 2-9 epilogue (TMEM -> bf16 / float32 -> shared memory ->
+// coalesced rows), warp 10 loads B, warp 11 zeroes row tails.  Two accumulators: the epilogue of a tile
 // overlaps the next tile's products.  Every wait is bounded as in tc.cu.
 #include <atomic>
 
@@ -56,14 +57,15 @@ constexpr int kHalf = 128;               // rows of A, and most rows of B, per C
 constexpr int kTileM = 2 * kHalf, kTileN = 2 * kHalf;
 constexpr int kOperandBytes = kHalf * kStageK * 2;  // 16 KB
 constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kRunStages = 8;            // stages of the weight gradient's sums per run (512 rows)
+constexpr int kRunStages = 12;           // stages of the weight gradient's sums per run (768 rows)
 constexpr int kChunkBytes = kStageK * 128;  // 64 columns x 64 terms of an M- or N-major operand
 constexpr int kEpiWarps = 8;             // two groups of four (one per TMEM lane quadrant), half the columns each
-constexpr int kThreads = (3 + kEpiWarps) * 32;
+constexpr int kThreads = (4 + kEpiWarps) * 32;
 constexpr int kTmemCols = 512;
 constexpr int kBandTiles = 8;            // row tiles per band of the unit order
 // epilogue staging, per group of warps two buffers of 16 rows x 128 bf16
-// (pitch 272 bytes), or per warp 32 rows x 32 float32 (pitch 144 bytes)
+// (pitch 272 bytes), or per warp 32 rows x 32 float32 (pitch 144 bytes), or per
+// warp 32 rows x 128 bytes for a TMA store (128-byte swizzle)
 constexpr int kChunkRows = 16;
 constexpr int kRowPitch = 272;
 constexpr int kRowBuf = kChunkRows * kRowPitch;
@@ -120,6 +122,45 @@ __device__ __forceinline__ void tma_pair(uint32_t dst, const CUtensorMap *map, i
         "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
         : "memory");
 }
+
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"((uint64_t)map),
+                 "r"(x), "r"(y), "r"(z), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// One lane of a converged warp.  The loading and issuing warps stay converged
+// and let one lane issue: with a branch on the lane number around the loop the
+// compiler cannot keep addresses and descriptors in uniform registers, and a
+// stage's four MMAs took 498 clocks to issue instead of fewer than the 512 that
+// they run (577 -> 514 clocks per stage).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(r));
+    return r != 0;
+}
+
+// The four MMAs of a stage: 16 terms each, a_step and b_step apart in the
+// operands' descriptors.
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ void mma_stage(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, t;\n\t"
+        "setp.ne.b32 p, %10, 0;\n\t"
+        "setp.eq.b32 t, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %9, p;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %3, %4, %9, t;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %5, %6, %9, t;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %7, %8, %9, t;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "l"(a + A_STEP), "l"(b + B_STEP), "l"(a + 2 * A_STEP), "l"(b + 2 * B_STEP),
+        "l"(a + 3 * A_STEP), "l"(b + 3 * B_STEP), "r"(idesc), "r"((uint32_t)accumulate));
+}
+static_assert(kStageK == 64, "four MMAs per stage");
 
 // Barriers 1 and 2: the epilogue's groups of four warps.
 __device__ __forceinline__ void epi_bar(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
@@ -222,8 +263,9 @@ struct Units {
 // The tensor maps of a launch.  a, b: the whole boxes (two 64-column chunks of
 // an M- or N-major operand); a_edge, b_edge: one chunk; b_rows: rows of a
 // K-major B in boxes of 32 and 64 rows.
+// out: dW, and parts the sums of a group's parts, 32 rows x 128 bytes.
 struct Maps {
-    CUtensorMap a, b, a_edge, b_edge, b_rows[2];
+    CUtensorMap a, b, a_edge, b_edge, b_rows[2], out, parts;
 };
 
 template <GroupedOp OP>
@@ -286,57 +328,47 @@ __global__ void __launch_bounds__(kThreads, 1)
     Units<OP> units{start, tiles, a.groups, m_tiles, a.inputs, a.outputs, a.part_rows};
     const int64_t total = units.total();
 
-    if (warp == 0) {
-        // ---------------- TMA
-        if (lane == 0) {
-            uint32_t j = 0;  // stages issued by this CTA
-            bool ok = true;
-            for (int64_t u = cluster; u < total && ok; u += n_clusters) {
-                const Unit w = units.at(u);
-                const int half_n = w.n >> 1;  // this CTA's rows (columns) of B
-                const int am = w.m0 + (int)rank * kHalf;
-                const int bn = w.n0 + (int)rank * half_n + (OP == kWeightGrad ? 0 : w.row0);
-                // an M- or N-major operand's two chunks in one box unless its last column cuts one
-                const int a_cols = OP == kInputGrad ? a.inputs : a.outputs;
-                const bool a_whole = OP == kProduct || am + kHalf <= (a_cols & ~63);
-                const bool b_whole = OP != kWeightGrad || (w.n == kTileN && bn + kHalf <= (a.inputs & ~63));
-                const int b_chunks = OP == kWeightGrad ? (half_n + 63) / 64 : 0;
-                // a K-major B by the smallest box that holds its rows
-                const CUtensorMap *b_map = OP == kWeightGrad || half_n > 64 ? &maps.b : &maps.b_rows[half_n > 32];
-                const uint32_t bytes =
-                    kOperandBytes + (OP == kWeightGrad ? b_chunks * kChunkBytes
-                                     : half_n > 64     ? kOperandBytes
-                                                       : (half_n > 32 ? 64 : 32) * 128);
-                for (int s = 0; s < w.stages; s++, j++) {
-                    const int sb = (int)(j % kStages);
-                    if (!wait_for(&empty[sb], ((j / kStages) & 1) ^ 1, ab, 1)) {
-                        ok = false;
-                        break;
-                    }
-                    const int k0 = s * kStageK;
-                    uint32_t bar;
-                    if (OP == kWeightGrad && k0 + kStageK > w.rows) {
+    if (warp == 0 || warp == 2 + kEpiWarps) {
+        // ---------------- TMA: A, and the arrival for both operands, or B
+        const bool loads_a = warp == 0;
+        const bool issuer = elect_one();
+        uint32_t j = 0;  // stages issued by this CTA
+        bool ok = true;
+        for (int64_t u = cluster; u < total && ok; u += n_clusters) {
+            const Unit w = units.at(u);
+            const int half_n = w.n >> 1;  // this CTA's rows (columns) of B
+            const int am = w.m0 + (int)rank * kHalf;
+            const int bn = w.n0 + (int)rank * half_n + (OP == kWeightGrad ? 0 : w.row0);
+            // an M- or N-major operand's two chunks in one box unless its last column cuts one
+            const int a_cols = OP == kInputGrad ? a.inputs : a.outputs;
+            const bool a_whole = OP == kProduct || am + kHalf <= (a_cols & ~63);
+            const bool b_whole = OP != kWeightGrad || (w.n == kTileN && bn + kHalf <= (a.inputs & ~63));
+            const int b_chunks = OP == kWeightGrad ? (half_n + 63) / 64 : 0;
+            // a K-major B by the smallest box that holds its rows
+            const CUtensorMap *b_map = OP == kWeightGrad || half_n > 64 ? &maps.b : &maps.b_rows[half_n > 32];
+            const uint32_t bytes =
+                kOperandBytes + (OP == kWeightGrad ? b_chunks * kChunkBytes
+                                 : half_n > 64     ? kOperandBytes
+                                                   : (half_n > 32 ? 64 : 32) * 128);
+            for (int s = 0; s < w.stages; s++, j++) {
+                const int sb = (int)(j % kStages);
+                ok = __all_sync(0xffffffffu, wait_for(&empty[sb], ((j / kStages) & 1) ^ 1, ab, 1));
+                if (!ok) break;
+                const int k0 = s * kStageK;
+                // B's bytes may land before the arrival below: the phase waits for it
+                const bool cut = OP == kWeightGrad && k0 + kStageK > w.rows;
+                if (loads_a && issuer) {
+                    if (cut) {
                         mbar_arrive_expect_tx(&tail[sb], bytes);
-                        bar = mapa_shared(smem_u32(&tail[sb]), rank);
-                    } else {
-                        if (leader) {
-                            mbar_arrive_expect_tx(&full[sb], 2 * bytes);
-                            mbar_arrive(&full[sb]);
-                        }
-                        bar = mapa_shared(smem_u32(&full[sb]), 0);
+                    } else if (leader) {
+                        mbar_arrive_expect_tx(&full[sb], 2 * bytes);
+                        mbar_arrive(&full[sb]);
                     }
-                    const uint32_t sa = smem_u32(smem + sb * kStageBytes), sbb = sa + kOperandBytes;
-                    if (OP == kProduct) {
-                        tma_pair(sa, &maps.a, k0, am, w.g, bar);
-                    } else if (a_whole) {
-                        if (OP == kInputGrad) tma_pair(sa, &maps.a, 0, k0, am / 64, w.g, bar);
-                        else tma_pair(sa, &maps.a, 0, w.row0 + k0, am / 64, bar);
-                    } else {
-                        for (int i = 0; i < 2; i++) {
-                            if (OP == kInputGrad) tma_pair(sa + i * kChunkBytes, &maps.a_edge, am + 64 * i, k0, w.g, bar);
-                            else tma_pair(sa + i * kChunkBytes, &maps.a_edge, am + 64 * i, w.row0 + k0, bar);
-                        }
-                    }
+                }
+                const uint32_t bar = cut ? mapa_shared(smem_u32(&tail[sb]), rank) : mapa_shared(smem_u32(&full[sb]), 0);
+                const uint32_t sa = smem_u32(smem + sb * kStageBytes), sbb = sa + kOperandBytes;
+                if (!issuer) {
+                } else if (!loads_a) {
                     if (OP != kWeightGrad) {
                         tma_pair(sbb, b_map, k0, bn, bar);
                     } else if (b_whole) {
@@ -345,13 +377,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < b_chunks; i++)
                             tma_pair(sbb + i * kChunkBytes, &maps.b_edge, bn + 64 * i, w.row0 + k0, bar);
                     }
+                } else if (OP == kProduct) {
+                    tma_pair(sa, &maps.a, k0, am, w.g, bar);
+                } else if (a_whole) {
+                    if (OP == kInputGrad) tma_pair(sa, &maps.a, 0, k0, am / 64, w.g, bar);
+                    else tma_pair(sa, &maps.a, 0, w.row0 + k0, am / 64, bar);
+                } else {
+                    for (int i = 0; i < 2; i++) {
+                        if (OP == kInputGrad) tma_pair(sa + i * kChunkBytes, &maps.a_edge, am + 64 * i, k0, w.g, bar);
+                        else tma_pair(sa + i * kChunkBytes, &maps.a_edge, am + 64 * i, w.row0 + k0, bar);
+                    }
                 }
+                __syncwarp();
             }
-            if (*ab.own) settle();
         }
+        if (*ab.own) settle();
     } else if (warp == 1) {
         // ---------------- MMA issue (leader)
-        if (leader && lane == 0) {
+        if (leader) {
+            const bool issuer = elect_one();
             uint32_t j = 0, run = 0;  // stages, and accumulators filled
             bool ok = true;
             for (int64_t u = cluster; u < total && ok; u += n_clusters) {
@@ -360,30 +404,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int run_stages = OP == kWeightGrad && a.sum_runs ? kRunStages : w.stages;
                 for (int s0 = 0; s0 < w.stages && ok; s0 += run_stages, run++) {
                     const uint32_t acc = run & 1, d = tmem_base + acc * kTileN;
-                    if (!wait_for(&tmem_empty[acc], ((run >> 1) & 1) ^ 1, ab, 2)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = __all_sync(0xffffffffu, wait_for(&tmem_empty[acc], ((run >> 1) & 1) ^ 1, ab, 2));
+                    if (!ok) break;
                     tc_fence_after();
                     const int s1 = min(w.stages, s0 + run_stages);
                     for (int s = s0; s < s1; s++, j++) {
                         const int sb = (int)(j % kStages);
-                        if (!wait_for(&full[sb], (j / kStages) & 1, ab, 3)) {
-                            ok = false;
-                            break;
-                        }
+                        ok = __all_sync(0xffffffffu, wait_for(&full[sb], (j / kStages) & 1, ab, 3));
+                        if (!ok) break;
                         tc_fence_after();
                         const uint32_t sa = smem_u32(smem + sb * kStageBytes), sbb = sa + kOperandBytes;
                         const uint64_t ad = OP == kProduct ? sw128_desc(sa) : column_major_desc(sa);
                         const uint64_t bd = OP == kWeightGrad ? column_major_desc(sbb) : sw128_desc(sbb);
-#pragma unroll
-                        for (int k = 0; k < kStageK / 16; k++)
+                        if (issuer) {
                             // 16 terms: 32 bytes of a K-major row, 16 rows of the others
-                            umma2_bf16(d, ad + k * (OP == kProduct ? 2 : 128), bd + k * (OP == kWeightGrad ? 128 : 2),
-                                       idesc, s > s0 || k > 0);
-                        umma2_commit_mc(&empty[sb], 0x3);
+                            mma_stage<OP == kProduct ? 2 : 128, OP == kWeightGrad ? 128 : 2>(d, ad, bd, idesc, s > s0);
+                            umma2_commit_mc(&empty[sb], 0x3);
+                        }
+                        __syncwarp();
                     }
-                    if (ok) umma2_commit_mc(&tmem_full[acc], 0x3);
+                    if (ok && issuer) umma2_commit_mc(&tmem_full[acc], 0x3);
+                    __syncwarp();
                 }
             }
             if (*ab.own) settle();
@@ -461,8 +502,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                     release(acc);
                 }
                 if (!ok) break;
-                float *stage = reinterpret_cast<float *>(epi) + (warp - 2) * 32 * kGradPitch;
                 const bool f32 = a.out_f32 || w.part >= 0, add = a.accumulate && w.part < 0;
+                if (!add) {
+                    // TMA writes the rows out, and leaves out what lies past the last row and column: the LSU path
+                    // below costs the shared memory that feeds the MMAs twice the traffic
+                    const uint32_t buf_addr = smem_u32(epi) + (warp - 2) * 4096;
+                    const int m0 = m_first + quad * 32, n0 = w.n0 + group * kHalf;
+                    const int per = f32 ? 32 : 64;  // columns in 128 bytes
+#pragma unroll
+                    for (int c = 0; c < kHalf / 32; c++) {
+                        if (c * per >= left || c * per >= kHalf || m0 >= a.outputs) break;
+                        // the last store has read the buffer
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            uint32_t x[4];
+                            if (f32) {
+#pragma unroll
+                                for (int q = 0; q < 4; q++) x[q] = __float_as_uint(sum[c * 32 + i * 4 + q]);
+                            } else {
+                                const int e = (c & 1) * 64 + i * 8;
+#pragma unroll
+                                for (int q = 0; q < 4; q++) x[q] = pack_bf16(sum[e + 2 * q], sum[e + 2 * q + 1]);
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf_addr + lane * 128 +
+                                                                                         ((i ^ (lane & 7)) << 4)),
+                                         "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                                         : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (elect_one())
+                            tma_store(w.part >= 0 ? &maps.parts : &maps.out, buf_addr, n0 + c * per, m0,
+                                      w.part >= 0 ? w.part : w.g);
+                    }
+                    continue;
+                }
+                float *stage = reinterpret_cast<float *>(epi) + (warp - 2) * 32 * kGradPitch;
                 void *base = w.part >= 0 ? (void *)a.parts : a.out;
                 const int64_t o0 = ((int64_t)(w.part >= 0 ? w.part : w.g) * a.outputs + m_first + quad * 32) * a.inputs +
                                    w.n0 + group * kHalf;
@@ -517,6 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
+        if (OP == kWeightGrad) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (OP == kWeightGrad) {
         // ---------------- rows past a group's end, in the sum's last stage, become zeros
         uint32_t j = 0, phases = 0;  // stages passed; per stage of the ring, the parity of its next tail
@@ -554,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// A bf16 view of `base` with 128-byte swizzle: axis i has size[i] elements
+// A bf16 (float32) view of `base` with 128-byte swizzle: axis i has size[i] elements
 // stride[i] elements apart (axis 0 one) and box[i] of them per box; what lies
 // outside the sizes reads as zeros.
 struct View {
@@ -562,7 +640,7 @@ struct View {
     int64_t size[4], stride[4];
     int box[4];
 };
-int encode_view(CUtensorMap *map, const void *base, const View &v) {
+int encode_view(CUtensorMap *map, const void *base, const View &v, bool f32 = false) {
     auto enc = tensor_map_encoder();
     if (!enc) return fail(GTMOE_ECUDA, "cuTensorMapEncodeTiled is not available");
     cuuint64_t dims[4], strides[3];
@@ -570,10 +648,11 @@ int encode_view(CUtensorMap *map, const void *base, const View &v) {
     for (int i = 0; i < v.axes; i++) {
         dims[i] = (cuuint64_t)v.size[i];
         boxes[i] = (cuuint32_t)v.box[i];
-        if (i) strides[i - 1] = (cuuint64_t)v.stride[i] * 2;
+        if (i) strides[i - 1] = (cuuint64_t)v.stride[i] * (f32 ? 4 : 2);
     }
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)v.axes, const_cast<void *>(base), dims,
-                           strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const CUresult r = enc(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                           (cuuint32_t)v.axes, const_cast<void *>(base), dims, strides, boxes, ones,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(GTMOE_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return 0;
@@ -668,6 +747,13 @@ int launch(const GroupedProduct &p, int device, cudaStream_t st) {
         GT_CHECK(encode_view(&m.b, p.b, chunks(rows, in)));
         GT_CHECK(encode_view(&m.b_edge, p.b, matrix(rows, in, kStageK)));
         m.b_rows[0] = m.b_rows[1] = m.b_edge;
+        const bool f32 = p.out_dtype == GTMOE_DTYPE_F32;
+        GT_CHECK(encode_view(&m.out, p.c, {3, {in, out, p.groups}, {1, in, in * out}, {f32 ? 32 : 64, 32, 1}}, f32));
+        m.parts = m.out;
+        const int part = part_rows(rows, in, out, p.groups);
+        if (part != kAnyRows)
+            GT_CHECK(encode_view(&m.parts, p.workspace,
+                                 {3, {in, out, rows / part + p.groups}, {1, in, in * out}, {32, 32, 1}}, true));
     } else {
         const int64_t sum = OP == kProduct ? in : out, group = in * out;
         if (OP == kProduct) {
@@ -681,7 +767,7 @@ int launch(const GroupedProduct &p, int device, cudaStream_t st) {
         GT_CHECK(encode_view(&m.b, p.a, matrix(rows, sum, kHalf)));
         GT_CHECK(encode_view(&m.b_rows[0], p.a, matrix(rows, sum, 32)));
         GT_CHECK(encode_view(&m.b_rows[1], p.a, matrix(rows, sum, 64)));
-        m.b_edge = m.b;
+        m.b_edge = m.out = m.parts = m.b;
     }
     DenseArgs a;
     a.counts = p.counts;
