@@ -11,16 +11,34 @@
 // their digits.  All sums have a fixed order: results repeat bit for bit.
 #include <math.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "operators.h"
+#include "sm100.cuh"
 
 namespace gtmoe {
 namespace {
 
-constexpr int kFwdThreads = 256;
-constexpr int kBwdThreads = 512;
+constexpr int kWideThreads = 256;
+constexpr int kRingThreads = 256;
 // Blocks of the backward, each of which leaves one row of partial weight and
 // bias gradients: two per SM of a B200.
 constexpr int kBwdBlocks = 2 * 148;
+// A ring's mbarriers and abort flag come before its stages in shared memory.
+constexpr int kMaxStages = 8;
+constexpr int kRingHeader = 256;
+// Shared memory for the stages of a backward's block of 256 threads (of 512:
+// twice this): two blocks per SM.
+constexpr int kBwdStageBytes = 98304;
+// The forward: warps per block, tiles in a warp's ring, and shared memory for
+// a block's rings.
+constexpr int kFwdMostWarps = 8;
+constexpr int kFwdStages = 2;
+constexpr int kFwdMostBytes = 200 * 1024;
+static_assert(2 * kMaxStages * 8 + 4 <= kRingHeader && kFwdMostWarps * (kFwdStages * 8 + 4) <= kRingHeader, "ring header");
+
+__device__ int g_norm_error;  // a bounded wait's code (gtmoe_operators_check)
 
 template <typename ACC>
 __device__ __forceinline__ ACC rsqrt_acc(ACC v);
@@ -45,11 +63,20 @@ __device__ __forceinline__ void team_sum(ACC (&v)[N], int team, int team_id, ACC
 #pragma unroll
         for (int i = 0; i < N; i++) red[warp][i] = v[i];
     asm volatile("bar.sync %0, %1;" ::"r"(1 + team_id), "r"(team) : "memory");
+    // (constant trip counts: the loads then overlap)
+    ACC (*mine)[N] = red + team_id * warps;
+    auto add_up = [&](auto count) {
 #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = red[team_id * warps][i];
-    for (int w = 1; w < warps; w++)
+        for (int i = 0; i < N; i++) v[i] = mine[0][i];
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] += red[team_id * warps + w][i];
+        for (int w = 1; w < decltype(count)::value; w++)
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] += mine[w][i];
+    };
+    if (warps == 8) add_up(std::integral_constant<int, 8>());
+    else if (warps == 4) add_up(std::integral_constant<int, 4>());
+    else if (warps == 2) add_up(std::integral_constant<int, 2>());
+    else add_up(std::integral_constant<int, 16>());
 }
 
 struct NormArgs {
@@ -58,7 +85,7 @@ struct NormArgs {
     int64_t rows;
     int width;
     double eps;
-    int team;
+    int team, stages;  // of the backward's ring
     // backward
     const void *dy, *dres;
     void *dx;
@@ -66,100 +93,391 @@ struct NormArgs {
     int want_params;
 };
 
-// A team per row; the row stays in NV vectors per thread.
-template <typename T, typename W, typename ACC, int VEC, int NV>
-__global__ void __launch_bounds__(kFwdThreads) norm_forward_kernel(const NormArgs a) {
-    using X = VecIO<T, ACC, VEC>;
-    using P = VecIO<W, ACC, VEC>;
-    __shared__ ACC red[2][kFwdThreads / 32][1];
-    const int team = a.team, team_id = threadIdx.x / team, tl = threadIdx.x - team_id * team;
-    const int teams = kFwdThreads / team, n = a.width;
-    const T *x = (const T *)a.x;
-    const W *w = (const W *)a.weight, *b = (const W *)a.bias;
-    for (int64_t row = (int64_t)blockIdx.x * teams + team_id; row < a.rows; row += (int64_t)gridDim.x * teams) {
-        const T *xr = x + row * n;
-        typename X::Raw raw[NV];
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * team + tl) * VEC;
-            if (c < n) raw[i] = X::load(xr + c);
+// ---- Rows on 16 bytes: tiles of consecutive rows stream through a ring of
+// shared-memory stages, filled by bulk copies a few tiles ahead, so that the
+// bytes in flight do not depend on how many registers the sums leave for
+// occupancy (the same kernels with rows loaded into registers reached 62 % of
+// the copy bandwidth).  A team of threads per row, NV vectors per thread.
+
+// Stage s of a block's ring: a tile's rows of each input one after another.
+template <typename T, int INPUTS>
+struct Ring {
+    uint8_t *data;
+    uint64_t *full, *empty;  // [stages]
+    int *abort_flag;
+    int stages, tile_rows, warps;
+    int given;  // inputs that are there: the first ones
+    int64_t rows, tiles;
+    int64_t row_bytes;
+    const void *in[INPUTS];
+
+    __device__ __forceinline__ const T *row(int stage, int input, int r) const {
+        return (const T *)(data + ((int64_t)(stage * given + input) * tile_rows + r) * row_bytes);
+    }
+    __device__ __forceinline__ void init() {
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < stages; s++) {
+                mbar_init(&full[s], 1);
+                mbar_init(&empty[s], warps);
+            }
+            *abort_flag = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        ACC s[1] = {ACC(0)};
+        __syncthreads();
+    }
+    // Thread 0: copies of tile `t` into its stage.
+    __device__ __forceinline__ void fill(int64_t t, int stage) {
+        const int64_t r0 = t * tile_rows;
+        const int64_t n = rows - r0 < tile_rows ? rows - r0 : tile_rows;
+        const uint32_t bytes = (uint32_t)(n * row_bytes);
+        mbar_arrive_expect_tx(&full[stage], bytes * given);
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * team + tl) * VEC;
-            if (c < n) {
-                ACC v[VEC];
-                X::unpack(raw[i], v);
-#pragma unroll
-                for (int q = 0; q < VEC; q++) s[0] += v[q];
+        for (int i = 0; i < INPUTS; i++)
+            if (i < given)
+                asm volatile(
+                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                        smem_u32(row(stage, i, 0))),
+                    "l"((const uint8_t *)in[i] + r0 * row_bytes), "r"(bytes), "r"(smem_u32(&full[stage]))
+                    : "memory");
+    }
+    __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, int code) {
+        return mbar_wait(bar, parity, (volatile int *)abort_flag, &g_norm_error, code);
+    }
+};
+
+// Walks the block's tiles: body(stage, tile) by every thread, the stage's data
+// ready.  After a wait that ran out the others no longer wait: every warp still
+// walks all tiles (on whatever the stages hold), so that the teams' barriers
+// stay matched.
+// Thread 0 refills a stage one tile after it was read, so that it rarely waits
+// for a slower warp.
+template <typename R, typename F>
+__device__ __forceinline__ void walk_tiles(R &ring, F body) {
+    const int64_t first = blockIdx.x, step = gridDim.x;
+    if (threadIdx.x == 0)
+        for (int s = 0; s < ring.stages && first + s * step < ring.tiles; s++) ring.fill(first + s * step, s);
+    int stage = 0;
+    uint32_t phase = 0;
+    int64_t i = 0;
+    for (int64_t t = first; t < ring.tiles; t += step, i++) {
+        if (threadIdx.x == 0 && i > 0) {
+            const int64_t next = first + (i - 1 + ring.stages) * step;
+            if (next < ring.tiles) {
+                const int before = stage == 0 ? ring.stages - 1 : stage - 1;
+                if (ring.wait(&ring.empty[before], stage == 0 ? phase ^ 1 : phase, 2)) ring.fill(next, before);
             }
         }
-        team_sum<1, ACC>(s, team, team_id, red[0]);
-        const ACC mean = s[0] / (ACC)n;
-        s[0] = ACC(0);
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * team + tl) * VEC;
-            if (c < n) {
-                ACC v[VEC];
-                X::unpack(raw[i], v);
-#pragma unroll
-                for (int q = 0; q < VEC; q++) s[0] += (v[q] - mean) * (v[q] - mean);
-            }
+        ring.wait(&ring.full[stage], phase, 1);
+        __syncwarp();
+        body(stage, t);
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[stage]);
+        if (++stage == ring.stages) {
+            stage = 0;
+            phase ^= 1;
         }
-        team_sum<1, ACC>(s, team, team_id, red[1]);
-        const ACC rstd = rsqrt_acc<ACC>(s[0] / (ACC)n + (ACC)a.eps);
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * team + tl) * VEC;
-            if (c < n) {
-                ACC v[VEC], pw[VEC], pb[VEC];
-                X::unpack(raw[i], v);
-                if (w) P::unpack(P::load(w + c), pw);
-                if (b) P::unpack(P::load(b + c), pb);
-#pragma unroll
-                for (int q = 0; q < VEC; q++) {
-                    ACC r = (v[q] - mean) * rstd;
-                    if (w) r *= pw[q];
-                    if (b) r += pb[q];
-                    v[q] = r;
-                }
-                X::store((T *)a.y + row * n + c, v);
-            }
-        }
-        if (tl == 0) {
-            if (a.mean) ((ACC *)a.mean)[row] = mean;
-            if (a.rstd) ((ACC *)a.rstd)[row] = rstd;
+    }
+    if (*(volatile int *)ring.abort_flag && threadIdx.x == 0) {
+        // copies in flight land before the block can leave
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {
         }
     }
 }
 
-// Rows too wide for registers: a block per row reads it three times (the
-// second and third time mostly from L2).
-template <typename T, typename W, typename ACC>
-__global__ void __launch_bounds__(kFwdThreads) norm_forward_wide_kernel(const NormArgs a) {
-    __shared__ ACC red[2][kFwdThreads / 32][1];
+template <typename T, int INPUTS>
+__device__ __forceinline__ Ring<T, INPUTS> make_ring(const NormArgs &a, uint8_t *smem) {
+    Ring<T, INPUTS> r;
+    r.stages = a.stages;
+    r.tile_rows = (int)blockDim.x / a.team;
+    r.warps = (int)blockDim.x >> 5;
+    r.rows = a.rows;
+    r.tiles = (a.rows + r.tile_rows - 1) / r.tile_rows;
+    r.row_bytes = (int64_t)a.width * (int64_t)sizeof(T);
+    r.full = (uint64_t *)smem;
+    r.empty = r.full + kMaxStages;
+    r.abort_flag = (int *)(r.empty + kMaxStages);
+    r.data = smem + kRingHeader;
+    return r;
+}
+
+// A warp per tile of RP rows, with a ring of its own: no warp waits for another
+// (a team of four warps per row spent more time in its two sums' barriers than
+// a warp on the row), and the bytes in flight are those of the ring.  The RP
+// rows share each read of the weights and their sums' latencies overlap.  The
+// row is read from shared memory for each of the three passes.
+template <typename T, typename W, typename ACC, int VEC, int RP>
+__global__ void __launch_bounds__(kFwdMostWarps * 32) norm_forward_kernel(const NormArgs a) {
+    using X = VecIO<T, ACC, VEC>;
+    using P = VecIO<W, ACC, VEC>;
+    constexpr int H = VEC / 2;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, n = a.width;
+    const int64_t row_bytes = (int64_t)n * (int64_t)sizeof(T), tile_bytes = row_bytes * RP;
+    uint64_t *full = (uint64_t *)smem + warp * kFwdStages;
+    int *abort_flag = (int *)((uint64_t *)smem + kFwdMostWarps * kFwdStages) + warp;
+    uint8_t *data = smem + kRingHeader + warp * kFwdStages * tile_bytes;
+    const int64_t tiles = (a.rows + RP - 1) / RP, step = (int64_t)gridDim.x * warps;
+    const int64_t first = (int64_t)blockIdx.x * warps + warp;
+    auto fill = [&](int64_t t, int stage) {
+        const int64_t r0 = t * RP;
+        const uint32_t bytes = (uint32_t)((a.rows - r0 < RP ? a.rows - r0 : RP) * row_bytes);
+        mbar_arrive_expect_tx(&full[stage], bytes);
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                smem_u32(data + stage * tile_bytes)),
+            "l"((const uint8_t *)a.x + r0 * row_bytes), "r"(bytes), "r"(smem_u32(&full[stage]))
+            : "memory");
+    };
+    if (lane == 0) {
+        for (int s = 0; s < kFwdStages; s++) mbar_init(&full[s], 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int s = 0; s < kFwdStages; s++)
+            if (first + s * step < tiles) fill(first + s * step, s);
+    }
+    __syncwarp();
+    const W *w = (const W *)a.weight, *b = (const W *)a.bias;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int64_t t = first; t < tiles; t += step) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, (volatile int *)abort_flag, &g_norm_error, 1))) break;
+        const int64_t row = t * RP;
+        // past the last row the stage holds an earlier tile, or nothing yet: worked on, not written
+        const int there = (int)min((int64_t)RP, a.rows - row);
+        const T *x = (const T *)(data + stage * tile_bytes);
+        Pair<ACC> v[H], s2[RP];
+        ACC s[RP], mean[RP], rstd[RP];
+        auto row_sums = [&]() {
+#pragma unroll
+            for (int r = 0; r < RP; r++) s[r] = s2[r].x + s2[r].y;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int r = 0; r < RP; r++) s[r] += __shfl_xor_sync(0xffffffffu, s[r], o);
+        };
+#pragma unroll
+        for (int r = 0; r < RP; r++) s2[r] = both(ACC(0));
+#pragma unroll (16 / RP)
+        for (int c = lane * VEC; c < n; c += 32 * VEC)
+#pragma unroll
+            for (int r = 0; r < RP; r++) {
+                X::unpack(X::load(x + r * n + c), &v[0].x);
+#pragma unroll
+                for (int q = 0; q < H; q++) s2[r] = add2(s2[r], v[q]);
+            }
+        row_sums();
+#pragma unroll
+        for (int r = 0; r < RP; r++) {
+            mean[r] = s[r] / (ACC)n;  // exact for a constant row whose sum is
+            s2[r] = both(ACC(0));
+        }
+#pragma unroll (16 / RP)
+        for (int c = lane * VEC; c < n; c += 32 * VEC)
+#pragma unroll
+            for (int r = 0; r < RP; r++) {
+                X::unpack(X::load(x + r * n + c), &v[0].x);
+#pragma unroll
+                for (int q = 0; q < H; q++) {
+                    const Pair<ACC> d = add2(v[q], both(-mean[r]));
+                    s2[r] = fma2(d, d, s2[r]);
+                }
+            }
+        row_sums();
+#pragma unroll
+        for (int r = 0; r < RP; r++) rstd[r] = rsqrt_acc<ACC>(s[r] / (ACC)n + (ACC)a.eps);
+        T *y = (T *)a.y + row * n;
+#pragma unroll 4
+        for (int c = lane * VEC; c < n; c += 32 * VEC) {
+            Pair<ACC> pw[H], pb[H];
+            if (w) P::unpack(P::load_ro(w + c), &pw[0].x);
+            if (b) P::unpack(P::load_ro(b + c), &pb[0].x);
+#pragma unroll
+            for (int r = 0; r < RP; r++) {
+                X::unpack(X::load(x + r * n + c), &v[0].x);
+#pragma unroll
+                for (int q = 0; q < H; q++) {
+                    v[q] = mul2(add2(v[q], both(-mean[r])), both(rstd[r]));
+                    if (w && b) v[q] = fma2(v[q], pw[q], pb[q]);
+                    else if (w) v[q] = mul2(v[q], pw[q]);
+                    else if (b) v[q] = add2(v[q], pb[q]);
+                }
+                if (r < there) X::store(y + (int64_t)r * n + c, &v[0].x);
+            }
+        }
+        if (lane < there) {
+            ACC m = mean[0], rs = rstd[0];
+#pragma unroll
+            for (int r = 1; r < RP; r++)
+                if (lane == r) m = mean[r], rs = rstd[r];
+            if (a.mean) ((ACC *)a.mean)[row + lane] = m;
+            if (a.rstd) ((ACC *)a.rstd)[row + lane] = rs;
+        }
+        __syncwarp();  // the stage has been read
+        if (lane == 0 && t + kFwdStages * step < tiles) fill(t + kFwdStages * step, stage);
+        if (++stage == kFwdStages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    if (*(volatile int *)abort_flag && lane == 0) {
+        // copies in flight land before the warp leaves
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {
+        }
+    }
+}
+
+// Every thread has the same columns of each of its rows, so that the weight
+// and bias gradients add up in registers; each block leaves one partial row of
+// both.
+template <typename T, typename W, typename ACC, int VEC, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) norm_backward_kernel(const NormArgs a) {
+    using X = VecIO<T, ACC, VEC>;
+    using P = VecIO<W, ACC, VEC>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ ACC red[2][THREADS / 32][2];
+    const int team = a.team, team_id = threadIdx.x / team, tl = threadIdx.x - team_id * team, n = a.width;
+    const ACC inv_n = ACC(1) / (ACC)n;
+    Ring<T, 3> ring = make_ring<T, 3>(a, smem);
+    ring.in[0] = a.dy;
+    ring.in[1] = a.x;
+    ring.in[2] = a.dres;
+    ring.given = a.dres ? 3 : 2;
+    ring.init();
+    const W *w = (const W *)a.weight;
+    constexpr int H = VEC / 2;
+    Pair<ACC> aw2[NV * H], ab2[NV * H], pw[NV * H];
+#pragma unroll
+    for (int i = 0; i < NV * H; i++) aw2[i] = ab2[i] = both(ACC(0)), pw[i] = both(ACC(1));
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * team + tl) * VEC;
+        if (w && c < n) P::unpack(P::load(w + c), &pw[i * H].x);
+    }
+    int it = 0;
+    // the next row's statistics are on their way while a row is worked on
+    const int64_t first = (int64_t)blockIdx.x * ring.tile_rows + team_id, row_step = (int64_t)gridDim.x * ring.tile_rows;
+    ACC next_mean = ACC(0), next_rstd = ACC(0);
+    if (first < a.rows) next_mean = ((const ACC *)a.mean)[first], next_rstd = ((const ACC *)a.rstd)[first];
+    walk_tiles(ring, [&](int stage, int64_t t) {
+        const int64_t row = t * ring.tile_rows + team_id;
+        if (row >= a.rows) return;
+        const T *dy = ring.row(stage, 0, team_id), *x = ring.row(stage, 1, team_id), *dres = ring.row(stage, 2, team_id);
+        const ACC rs = next_rstd, mean = next_mean;
+        if (row + row_step < a.rows) {
+            next_mean = ((const ACC *)a.mean)[row + row_step];
+            next_rstd = ((const ACC *)a.rstd)[row + row_step];
+        }
+        Pair<ACC> s1 = both(ACC(0)), s2 = both(ACC(0)), g[NV * H], xh[NV * H];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * team + tl) * VEC;
+            if (c < n) {
+                X::unpack(X::load(x + c), &xh[i * H].x);
+                X::unpack(X::load(dy + c), &g[i * H].x);
+#pragma unroll
+                for (int e = i * H; e < (i + 1) * H; e++) {
+                    xh[e] = mul2(add2(xh[e], both(-mean)), both(rs));
+                    aw2[e] = fma2(g[e], xh[e], aw2[e]);
+                    ab2[e] = add2(ab2[e], g[e]);
+                    g[e] = mul2(g[e], pw[e]);
+                    s1 = add2(s1, g[e]);
+                    s2 = fma2(g[e], xh[e], s2);
+                }
+            }
+        }
+        ACC s[2] = {s1.x + s1.y, s2.x + s2.y};
+        team_sum<2, ACC>(s, team, team_id, red[it]);
+        it ^= 1;
+        // dx = rs g - rs m1 - xh rs m2 (+ dres)
+        const ACC c1 = -rs * (s[0] * inv_n), c2 = -rs * (s[1] * inv_n);
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * team + tl) * VEC;
+            if (c < n) {
+                Pair<ACC> v[H];
+                if (a.dres) X::unpack(X::load(dres + c), &v[0].x);
+#pragma unroll
+                for (int q = 0; q < H; q++) {
+                    const int e = i * H + q;
+                    const Pair<ACC> d = fma2(both(rs), g[e], fma2(xh[e], both(c2), both(c1)));
+                    v[q] = a.dres ? add2(v[q], d) : d;
+                }
+                X::store((T *)a.dx + row * n + c, &v[0].x);
+            }
+        }
+    });
+    const ACC *aw = &aw2[0].x, *ab = &ab2[0].x;
+    if (!a.want_params) return;
+    ACC *out = (ACC *)a.partial + (int64_t)blockIdx.x * 2 * n;
+    // the teams' sums in team order, in the ring's memory (its copies have all been waited for)
+    ACC *total = (ACC *)(smem + kRingHeader);
+    const int teams = (int)blockDim.x / team;
+    for (int t = 0; t < teams; t++) {
+        __syncthreads();
+        if (team_id == t) {
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int q = 0; q < VEC; q++) {
+                    const int c = (i * team + tl) * VEC + q, e = i * VEC + q;
+                    if (c < n) {
+                        const ACC sw = t ? total[c] + aw[e] : aw[e], sb = t ? total[n + c] + ab[e] : ab[e];
+                        if (t == teams - 1) {
+                            out[c] = sw;
+                            out[n + c] = sb;
+                        } else {
+                            total[c] = sw;
+                            total[n + c] = sb;
+                        }
+                    }
+                }
+        }
+    }
+}
+
+// ---- Any other row: a block per row reads it three times (the second and
+// third time mostly from L1 and L2).
+template <typename T, typename W, typename ACC, int VEC>
+__global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const NormArgs a) {
+    using X = VecIO<T, ACC, VEC>;
+    using P = VecIO<W, ACC, VEC>;
+    __shared__ ACC red[2][kWideThreads / 32][1];
     const int n = a.width;
     const W *w = (const W *)a.weight, *b = (const W *)a.bias;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *xr = (const T *)a.x + row * n;
-        ACC s[1] = {ACC(0)};
-        for (int c = threadIdx.x; c < n; c += kFwdThreads) s[0] += (ACC)xr[c];
-        team_sum<1, ACC>(s, kFwdThreads, 0, red[0]);
+        ACC s[1] = {ACC(0)}, v[VEC];
+#pragma unroll 4
+        for (int64_t c = threadIdx.x * VEC; c < n; c += kWideThreads * VEC) {
+            X::unpack(X::load(xr + c), v);
+#pragma unroll
+            for (int q = 0; q < VEC; q++) s[0] += v[q];
+        }
+        team_sum<1, ACC>(s, kWideThreads, 0, red[0]);
         const ACC mean = s[0] / (ACC)n;
         s[0] = ACC(0);
-        for (int c = threadIdx.x; c < n; c += kFwdThreads) {
-            const ACC v = (ACC)xr[c] - mean;
-            s[0] += v * v;
+#pragma unroll 4
+        for (int64_t c = threadIdx.x * VEC; c < n; c += kWideThreads * VEC) {
+            X::unpack(X::load(xr + c), v);
+#pragma unroll
+            for (int q = 0; q < VEC; q++) s[0] += (v[q] - mean) * (v[q] - mean);
         }
-        team_sum<1, ACC>(s, kFwdThreads, 0, red[1]);
+        team_sum<1, ACC>(s, kWideThreads, 0, red[1]);
         const ACC rstd = rsqrt_acc<ACC>(s[0] / (ACC)n + (ACC)a.eps);
-        for (int c = threadIdx.x; c < n; c += kFwdThreads) {
-            ACC r = ((ACC)xr[c] - mean) * rstd;
-            if (w) r *= (ACC)w[c];
-            if (b) r += (ACC)b[c];
-            ((T *)a.y)[row * n + c] = (T)r;
+        for (int64_t c = threadIdx.x * VEC; c < n; c += kWideThreads * VEC) {
+            ACC pw[VEC], pb[VEC];
+            X::unpack(X::load(xr + c), v);
+            if (w) P::unpack(P::load(w + c), pw);
+            if (b) P::unpack(P::load(b + c), pb);
+#pragma unroll
+            for (int q = 0; q < VEC; q++) {
+                v[q] = (v[q] - mean) * rstd;
+                if (w) v[q] *= pw[q];
+                if (b) v[q] += pb[q];
+            }
+            X::store((T *)a.y + row * n + c, v);
         }
         if (threadIdx.x == 0) {
             if (a.mean) ((ACC *)a.mean)[row] = mean;
@@ -168,253 +486,249 @@ __global__ void __launch_bounds__(kFwdThreads) norm_forward_wide_kernel(const No
     }
 }
 
-// One team per row, every thread the same columns of each of its rows, so
-// that the weight and bias gradients add up in registers; each block leaves
-// one partial row of both.
+// The backward of any other row: read twice; a thread adds its columns'
+// gradients into the block's partial row in memory, or for narrow rows
+// (width <= NV * kWideThreads, VEC 1) in registers.
 template <typename T, typename W, typename ACC, int VEC, int NV>
-__global__ void __launch_bounds__(kBwdThreads) norm_backward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(const NormArgs a) {
     using X = VecIO<T, ACC, VEC>;
     using P = VecIO<W, ACC, VEC>;
-    __shared__ ACC red[2][kBwdThreads / 32][2];
-    __shared__ ACC total[2][kBwdThreads / 2 * VEC * (VEC == 1 ? NV : 1)];
-    const int team = a.team, team_id = threadIdx.x / team, tl = threadIdx.x - team_id * team;
-    const int teams = kBwdThreads / team, n = a.width;
-    const ACC inv_n = ACC(1) / (ACC)n;
-    const T *x = (const T *)a.x, *dy = (const T *)a.dy, *dres = (const T *)a.dres;
-    const W *w = (const W *)a.weight;
-    ACC aw[NV * VEC], ab[NV * VEC];
-#pragma unroll
-    for (int i = 0; i < NV * VEC; i++) aw[i] = ab[i] = ACC(0);
-    const int64_t step = (int64_t)gridDim.x * teams;
-    int64_t row = (int64_t)blockIdx.x * teams + team_id;
-    typename X::Raw nx[NV], ng[NV];
-    ACC mean = ACC(0), rstd = ACC(0);
-    auto fetch = [&](int64_t r) {
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * team + tl) * VEC;
-            if (c < n) {
-                nx[i] = X::load(x + r * n + c);
-                ng[i] = X::load(dy + r * n + c);
-            }
-        }
-        mean = ((const ACC *)a.mean)[r];
-        rstd = ((const ACC *)a.rstd)[r];
-    };
-    if (row < a.rows) fetch(row);
-    for (int it = 0; row < a.rows; row += step, it ^= 1) {
-        ACC g[NV * VEC], xh[NV * VEC];
-        const ACC rs = rstd;
-        ACC s[2] = {ACC(0), ACC(0)};
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * team + tl) * VEC;
-            if (c < n) {
-                ACC pw[VEC];
-                X::unpack(nx[i], xh + i * VEC);
-                X::unpack(ng[i], g + i * VEC);
-                if (w) P::unpack(P::load(w + c), pw);
-#pragma unroll
-                for (int q = 0; q < VEC; q++) {
-                    const int e = i * VEC + q;
-                    xh[e] = (xh[e] - mean) * rs;
-                    aw[e] += g[e] * xh[e];
-                    ab[e] += g[e];
-                    if (w) g[e] *= pw[q];
-                    s[0] += g[e];
-                    s[1] += g[e] * xh[e];
-                }
-            }
-        }
-        if (row + step < a.rows) fetch(row + step);  // in flight while the team's sums are made
-        typename X::Raw rr[NV];
-        if (dres) {
-#pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const int c = (i * team + tl) * VEC;
-                if (c < n) rr[i] = X::load(dres + row * n + c);
-            }
-        }
-        team_sum<2, ACC>(s, team, team_id, red[it]);
-        const ACC m1 = s[0] * inv_n, m2 = s[1] * inv_n;
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * team + tl) * VEC;
-            if (c < n) {
-                ACC v[VEC];
-                if (dres) X::unpack(rr[i], v);
-#pragma unroll
-                for (int q = 0; q < VEC; q++) {
-                    const int e = i * VEC + q;
-                    const ACC d = rs * (g[e] - m1 - xh[e] * m2);
-                    v[q] = dres ? v[q] + d : d;
-                }
-                X::store((T *)a.dx + row * n + c, v);
-            }
-        }
-    }
-    if (!a.want_params) return;
-    ACC *out = (ACC *)a.partial + (int64_t)blockIdx.x * 2 * n;
-    if (teams == 1) {
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-#pragma unroll
-            for (int q = 0; q < VEC; q++) {
-                const int c = (i * team + tl) * VEC + q;
-                if (c < n) {
-                    out[c] = aw[i * VEC + q];
-                    out[n + c] = ab[i * VEC + q];
-                }
-            }
-        return;
-    }
-    // several teams (so at most half the block each): their sums in team order
-    for (int t = 0; t < teams; t++) {
-        if (team_id == t) {
-#pragma unroll
-            for (int i = 0; i < (VEC == 1 ? NV : 1); i++)
-#pragma unroll
-                for (int q = 0; q < VEC; q++) {
-                    const int c = (i * team + tl) * VEC + q;
-                    if (c < n) {
-                        total[0][c] = t ? total[0][c] + aw[i * VEC + q] : aw[i * VEC + q];
-                        total[1][c] = t ? total[1][c] + ab[i * VEC + q] : ab[i * VEC + q];
-                    }
-                }
-        }
-        __syncthreads();
-    }
-    for (int c = threadIdx.x; c < n; c += kBwdThreads) {
-        out[c] = total[0][c];
-        out[n + c] = total[1][c];
-    }
-}
-
-// Rows too wide for registers: a block per row, read twice; a thread adds its
-// columns' gradients into the block's partial row in memory.
-template <typename T, typename W, typename ACC>
-__global__ void __launch_bounds__(kBwdThreads) norm_backward_wide_kernel(const NormArgs a) {
-    __shared__ ACC red[2][kBwdThreads / 32][2];
+    __shared__ ACC red[2][kWideThreads / 32][2];
     const int n = a.width;
     const ACC inv_n = ACC(1) / (ACC)n;
     const W *w = (const W *)a.weight;
     ACC *out = (ACC *)a.partial + (int64_t)blockIdx.x * 2 * n;
+    ACC aw[NV ? NV : 1] = {}, ab[NV ? NV : 1] = {};
     int it = 0;
     bool first = true;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, it ^= 1) {
         const T *x = (const T *)a.x + row * n, *dy = (const T *)a.dy + row * n;
+        T *dx = (T *)a.dx + row * n;
         const ACC mean = ((const ACC *)a.mean)[row], rs = ((const ACC *)a.rstd)[row];
         ACC s[2] = {ACC(0), ACC(0)};
-        for (int c = threadIdx.x; c < n; c += kBwdThreads) {
-            const ACC g = w ? (ACC)dy[c] * (ACC)w[c] : (ACC)dy[c];
-            s[0] += g;
-            s[1] += g * (((ACC)x[c] - mean) * rs);
-        }
-        team_sum<2, ACC>(s, kBwdThreads, 0, red[it]);
-        const ACC m1 = s[0] * inv_n, m2 = s[1] * inv_n;
-        for (int c = threadIdx.x; c < n; c += kBwdThreads) {
-            const ACC d = (ACC)dy[c], xh = ((ACC)x[c] - mean) * rs;
-            const ACC g = w ? d * (ACC)w[c] : d;
-            ACC v = rs * (g - m1 - xh * m2);
-            if (a.dres) v = (ACC)((const T *)a.dres)[row * n + c] + v;
-            ((T *)a.dx)[row * n + c] = (T)v;
-            if (a.want_params) {
-                out[c] = (first ? ACC(0) : out[c]) + d * xh;
-                out[n + c] = (first ? ACC(0) : out[n + c]) + d;
+        auto sums = [&](int64_t c, ACC *g, ACC *xh) {
+            ACC pw[VEC];
+            X::unpack(X::load(x + c), xh);
+            X::unpack(X::load(dy + c), g);
+            if (w) P::unpack(P::load(w + c), pw);
+#pragma unroll
+            for (int q = 0; q < VEC; q++) {
+                xh[q] = (xh[q] - mean) * rs;
+                if (w) g[q] *= pw[q];
+                s[0] += g[q];
+                s[1] += g[q] * xh[q];
+            }
+        };
+        if constexpr (NV > 0) {
+            // VEC 1: the row's values stay in registers
+            ACC g[NV], xh[NV], d[NV];
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int64_t c = threadIdx.x + i * kWideThreads;
+                if (c < n) {
+                    d[i] = (ACC)dy[c];
+                    sums(c, g + i, xh + i);
+                    aw[i] += d[i] * xh[i];
+                    ab[i] += d[i];
+                }
+            }
+            team_sum<2, ACC>(s, kWideThreads, 0, red[it]);
+            const ACC c1 = -rs * (s[0] * inv_n), c2 = -rs * (s[1] * inv_n);
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int64_t c = threadIdx.x + i * kWideThreads;
+                if (c < n) {
+                    ACC v = rs * g[i] + (xh[i] * c2 + c1);
+                    if (a.dres) v = (ACC)((const T *)a.dres)[row * n + c] + v;
+                    dx[c] = (T)v;
+                }
+            }
+        } else {
+            ACC g[VEC], xh[VEC], v[VEC], o[VEC];
+#pragma unroll 2
+            for (int64_t c = threadIdx.x * VEC; c < n; c += kWideThreads * VEC) sums(c, g, xh);
+            team_sum<2, ACC>(s, kWideThreads, 0, red[it]);
+            const ACC c1 = -rs * (s[0] * inv_n), c2 = -rs * (s[1] * inv_n);
+            for (int64_t c = threadIdx.x * VEC; c < n; c += kWideThreads * VEC) {
+                ACC d[VEC], pw[VEC];
+                X::unpack(X::load(x + c), xh);
+                X::unpack(X::load(dy + c), d);
+                if (w) P::unpack(P::load(w + c), pw);
+                if (a.dres) X::unpack(X::load((const T *)a.dres + row * n + c), o);
+#pragma unroll
+                for (int q = 0; q < VEC; q++) {
+                    xh[q] = (xh[q] - mean) * rs;
+                    v[q] = rs * (w ? d[q] * pw[q] : d[q]) + (xh[q] * c2 + c1);
+                    if (a.dres) v[q] = o[q] + v[q];
+                }
+                X::store(dx + c, v);
+                if (a.want_params)
+#pragma unroll
+                    for (int q = 0; q < VEC; q++) {
+                        out[c + q] = (first ? ACC(0) : out[c + q]) + d[q] * xh[q];
+                        out[n + c + q] = (first ? ACC(0) : out[n + c + q]) + d[q];
+                    }
             }
         }
         first = false;
     }
-}
-
-// The blocks' partial rows to the weight and bias gradients: 32 columns per
-// block, 16 runs of partial rows side by side, added in a fixed order.
-template <typename W, typename ACC>
-__global__ void __launch_bounds__(512) norm_params_kernel(const ACC *__restrict__ partial, int blocks, int n,
-                                                          void *dweight, void *dbias, int accumulate) {
-    __shared__ ACC sum[2][16][32];
-    const int c = blockIdx.x * 32 + threadIdx.x, run = threadIdx.y;
-    ACC s0 = ACC(0), s1 = ACC(0);
-    if (c < n)
-        for (int p = run; p < blocks; p += 16) {
-            s0 += partial[(int64_t)p * 2 * n + c];
-            s1 += partial[(int64_t)p * 2 * n + n + c];
+    if (NV > 0 && a.want_params)
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int64_t c = threadIdx.x + i * kWideThreads;
+            if (c < n) {
+                out[c] = aw[i];
+                out[n + c] = ab[i];
+            }
         }
-    sum[0][run][threadIdx.x] = s0;
-    sum[1][run][threadIdx.x] = s1;
-    __syncthreads();
-    if (run >= 2 || c >= n) return;
-    W *dst = (W *)(run == 0 ? dweight : dbias);
-    if (!dst) return;
-    ACC s = sum[run][0][threadIdx.x];
-    for (int r = 1; r < 16; r++) s += sum[run][r][threadIdx.x];
-    if (accumulate) s += (ACC)dst[c];
-    dst[c] = (W)s;
 }
 
-// Threads per row: the fewest (a power of two from 32 on) that hold the row
-// in nv vectors each.
-int team_for(int64_t vectors, int nv, int most) {
-    int team = 32;
-    while (team < most && (int64_t)team * nv < vectors) team *= 2;
-    return team;
+// The blocks' partial rows to the weight (blockIdx.y 0) and bias gradients: 32
+// columns per block, 32 runs of partial rows side by side, added in a fixed
+// order.  Launched while the backward still runs; it waits for its end.
+template <typename W, typename ACC>
+__global__ void __launch_bounds__(1024) norm_params_kernel(const ACC *__restrict__ partial, int blocks, int n,
+                                                           void *dweight, void *dbias, int accumulate) {
+    __shared__ ACC sum[32][33];
+    const int c = blockIdx.x * 32 + threadIdx.x, run = threadIdx.y;
+    W *dst = (W *)(blockIdx.y == 0 ? dweight : dbias);
+    const ACC *src = partial + blockIdx.y * (int64_t)n + c;
+    cudaGridDependencySynchronize();
+    ACC s = ACC(0);
+    if (c < n && dst) {
+#pragma unroll 5
+        for (int p = run; p < blocks; p += 32) s += src[(int64_t)p * 2 * n];
+    }
+    sum[run][threadIdx.x] = s;
+    __syncthreads();
+    // warp `run` now adds column run of the block
+    s = sum[threadIdx.x][run];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int column = blockIdx.x * 32 + run;
+    if (threadIdx.x == 0 && column < n && dst) {
+        if (accumulate) s += (ACC)dst[column];
+        dst[column] = (W)s;
+    }
+}
+
+// How a ring kernel runs: threads per row (the fewest, a power of two from 32
+// on, that hold the row in nv vectors each), rows per tile, stages.
+struct RingPlan {
+    int team, threads, stages, nv, smem;
+};
+// bytes: of a row, all inputs together; budget: shared memory for the stages
+// of a block of 256 threads
+bool ring_plan(int64_t vectors, int nv, int64_t bytes, int most_threads, int64_t budget, RingPlan *p) {
+    p->nv = nv;
+    p->team = 32;
+    while ((int64_t)p->team * nv < vectors) p->team *= 2;
+    if (p->team > most_threads) return false;
+    p->threads = p->team > kRingThreads ? p->team : kRingThreads;
+    const int64_t stage = bytes * (p->threads / p->team);
+    const int64_t fit = budget * (p->threads / kRingThreads) / stage;
+    p->stages = (int)(fit < kMaxStages ? fit : kMaxStages);
+    p->smem = (int)(kRingHeader + p->stages * stage);
+    return p->stages >= 2;
+}
+
+// Blocks of `kern` that fit on the device at once; `known` keeps the last
+// answer (device, shared memory, blocks).
+int resident_blocks(const void *kern, int threads, int smem, int most_smem, int device, std::atomic<uint64_t> &known,
+                    int64_t *blocks) {
+    const uint64_t key = ((uint64_t)(device + 1) << 52) | ((uint64_t)smem << 32);
+    const uint64_t v = known.load(std::memory_order_relaxed);
+    if ((v & ~(uint64_t)0xffffffffu) == key) {
+        *blocks = (int64_t)(v & 0xffffffffu);
+        return 0;
+    }
+    int per = 0, sms = 0;
+    GT_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem));
+    GT_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, smem));
+    GT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    if (per < 1) return fail(GTMOE_ECUDA, "layer norm: no block fits on this device");
+    *blocks = (int64_t)per * sms;
+    known.store(key | (uint64_t)*blocks, std::memory_order_relaxed);
+    return 0;
 }
 
 template <typename T, typename W, typename ACC, int VEC>
-int forward_vec(NormArgs a, cudaStream_t st) {
-    const int64_t vectors = ((int64_t)a.width + VEC - 1) / VEC;
-    // a row in one warp as far as 8 vectors per lane go (no barrier), in a
-    // larger team beyond
-    const int nv = vectors <= 64 ? 2 : 8;
-    if (vectors > (int64_t)kFwdThreads * 8) {
-        norm_forward_wide_kernel<T, W, ACC>
-            <<<(unsigned)(a.rows < 65535 ? a.rows : 65535), kFwdThreads, 0, st>>>(a);
-    } else {
-        a.team = team_for(vectors, nv, kFwdThreads);
-        const int64_t teams = kFwdThreads / a.team;
-        const int64_t want = (a.rows + teams - 1) / teams;
-        const unsigned grid = (unsigned)(want < 0x7fffffff ? want : 0x7fffffff);
-        if (nv == 2) norm_forward_kernel<T, W, ACC, VEC, 2><<<grid, kFwdThreads, 0, st>>>(a);
-        else norm_forward_kernel<T, W, ACC, VEC, 8><<<grid, kFwdThreads, 0, st>>>(a);
+int forward_vec(NormArgs a, int device, cudaStream_t st) {
+    if constexpr (VEC > 1) {
+        const int64_t bytes = (int64_t)a.width * sizeof(T);
+        // rows per warp: tiles of up to 8 KB, as long as every SM's warps get one
+        int rp = bytes <= 2048 ? 4 : bytes <= 4096 ? 2 : 1;
+        while (rp > 1 && a.rows < (int64_t)rp * 148 * 12) rp /= 2;
+        // small tiles: blocks of four warps, three or more per SM; large ones: one block of what fits
+        const int64_t ring = bytes * rp * kFwdStages, fit = kFwdMostBytes / ring;
+        if (fit >= 2) {
+            static std::atomic<uint64_t> known[3];
+            auto kern = rp == 4   ? norm_forward_kernel<T, W, ACC, VEC, 4>
+                        : rp == 2 ? norm_forward_kernel<T, W, ACC, VEC, 2>
+                                  : norm_forward_kernel<T, W, ACC, VEC, 1>;
+            const int warps = fit >= 12 ? 4 : fit < kFwdMostWarps ? (int)fit : kFwdMostWarps;
+            const int smem = (int)(kRingHeader + ring * warps);
+            const int64_t tiles = (a.rows + rp - 1) / rp, want = (tiles + warps - 1) / warps;
+            int64_t blocks = 0;
+            GT_CHECK(resident_blocks((const void *)kern, warps * 32, smem, kRingHeader + kFwdMostBytes, device,
+                                     known[rp / 2], &blocks));
+            kern<<<(unsigned)(want < blocks ? want : blocks), warps * 32, smem, st>>>(a);
+            GT_CUDA(cudaGetLastError());
+            note_launches(1);
+            return 0;
+        }
     }
+    norm_forward_wide_kernel<T, W, ACC, VEC><<<(unsigned)(a.rows < 148 * 64 ? a.rows : 148 * 64), kWideThreads, 0, st>>>(a);
     GT_CUDA(cudaGetLastError());
     note_launches(1);
     return 0;
 }
 
 template <typename T, typename W, typename ACC, int VEC>
-int backward_vec(NormArgs a, void *dweight, void *dbias, int accumulate, cudaStream_t st) {
-    const int64_t vectors = ((int64_t)a.width + VEC - 1) / VEC;
-    int64_t blocks;
-    if (a.rows == 0) {
-        blocks = 0;
-    } else if (vectors > (int64_t)kBwdThreads * (VEC == 1 ? 8 : 4)) {
-        blocks = a.rows < kBwdBlocks ? a.rows : kBwdBlocks;
-        norm_backward_wide_kernel<T, W, ACC><<<(unsigned)blocks, kBwdThreads, 0, st>>>(a);
-    } else {
-        const int most = VEC == 1 ? 2 : 1;  // vectors per thread below a whole block per row
-        a.team = team_for(vectors, most, kBwdThreads);
-        const int64_t teams = kBwdThreads / a.team, want = (a.rows + teams - 1) / teams;
-        blocks = want < kBwdBlocks ? want : kBwdBlocks;
-        const int64_t nv = (vectors + a.team - 1) / a.team;
-        const unsigned grid = (unsigned)blocks;
-        if constexpr (VEC == 1) {
-            if (nv <= 2) norm_backward_kernel<T, W, ACC, 1, 2><<<grid, kBwdThreads, 0, st>>>(a);
-            else norm_backward_kernel<T, W, ACC, 1, 8><<<grid, kBwdThreads, 0, st>>>(a);
-        } else {
-            if (nv <= 1) norm_backward_kernel<T, W, ACC, VEC, 1><<<grid, kBwdThreads, 0, st>>>(a);
-            else if (nv <= 2) norm_backward_kernel<T, W, ACC, VEC, 2><<<grid, kBwdThreads, 0, st>>>(a);
-            else norm_backward_kernel<T, W, ACC, VEC, 4><<<grid, kBwdThreads, 0, st>>>(a);
+int backward_vec(NormArgs a, void *dweight, void *dbias, int accumulate, int device, cudaStream_t st) {
+    int64_t blocks = 0;
+    if (a.rows > 0) {
+        RingPlan p;
+        bool ring = false;
+        if constexpr (VEC > 1) {
+            const int64_t vectors = a.width / VEC, bytes = (int64_t)a.width * sizeof(T) * (a.dres ? 3 : 2);
+            static std::atomic<uint64_t> known[3];
+            ring = ring_plan(vectors, vectors <= 32 ? 1 : 2, bytes, 512, kBwdStageBytes, &p);
+            if (ring) {
+                auto kern = p.nv == 1          ? norm_backward_kernel<T, W, ACC, VEC, 1, 256>
+                            : p.threads == 256 ? norm_backward_kernel<T, W, ACC, VEC, 2, 256>
+                                               : norm_backward_kernel<T, W, ACC, VEC, 2, 512>;
+                a.team = p.team;
+                a.stages = p.stages;
+                const int64_t rows = p.threads / p.team, tiles = (a.rows + rows - 1) / rows;
+                GT_CHECK(resident_blocks((const void *)kern, p.threads, p.smem, kRingHeader + 2 * kBwdStageBytes, device,
+                                         known[p.threads > 256 ? 2 : p.nv - 1], &blocks));
+                if (blocks > kBwdBlocks) blocks = kBwdBlocks;
+                if (blocks > tiles) blocks = tiles;
+                kern<<<(unsigned)blocks, p.threads, p.smem, st>>>(a);
+            }
         }
-    }
-    if (blocks) {
+        if (!ring) {
+            blocks = a.rows < kBwdBlocks ? a.rows : kBwdBlocks;
+            if (VEC == 1 && a.width <= 4 * kWideThreads)
+                norm_backward_wide_kernel<T, W, ACC, 1, 4><<<(unsigned)blocks, kWideThreads, 0, st>>>(a);
+            else norm_backward_wide_kernel<T, W, ACC, VEC, 0><<<(unsigned)blocks, kWideThreads, 0, st>>>(a);
+        }
         GT_CUDA(cudaGetLastError());
         note_launches(1);
     }
     if (!a.want_params) return 0;
-    norm_params_kernel<W, ACC><<<(unsigned)((a.width + 31) / 32), dim3(32, 16), 0, st>>>(
-        (const ACC *)a.partial, (int)blocks, a.width, dweight, dbias, accumulate);
-    GT_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.width + 31) / 32), 2);
+    cfg.blockDim = dim3(32, 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = blocks ? 1 : 0;
+    GT_CUDA(cudaLaunchKernelEx(&cfg, norm_params_kernel<W, ACC>, (const ACC *)a.partial, (int)blocks, (int)a.width,
+                               dweight, dbias, accumulate));
     note_launches(1);
     return 0;
 }
@@ -436,6 +750,13 @@ int64_t norm_workspace(int dtype, int64_t rows, int64_t width) {
 }
 
 }  // namespace
+
+int norm_take_error(int *code) {
+    const int zero = 0;
+    GT_CUDA(cudaMemcpyFromSymbol(code, g_norm_error, sizeof(int)));
+    if (*code) GT_CUDA(cudaMemcpyToSymbol(g_norm_error, &zero, sizeof(int)));
+    return 0;
+}
 
 }  // namespace gtmoe
 
@@ -469,14 +790,16 @@ int gtmoe_layer_norm(const void *x, int dtype, int64_t rows, int64_t width, cons
     const int vec = 16 / (int)dtype_size(dtype);
     const bool wide = width % vec == 0 && aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias);
     if (dtype == GTMOE_DTYPE_F64)
-        return wide ? forward_vec<double, double, double, 2>(a, st) : forward_vec<double, double, double, 1>(a, st);
+        return wide ? forward_vec<double, double, double, 2>(a, scope.device(), st)
+                    : forward_vec<double, double, double, 1>(a, scope.device(), st);
     if (dtype == GTMOE_DTYPE_F32)
-        return wide ? forward_vec<float, float, float, 4>(a, st) : forward_vec<float, float, float, 1>(a, st);
+        return wide ? forward_vec<float, float, float, 4>(a, scope.device(), st)
+                    : forward_vec<float, float, float, 1>(a, scope.device(), st);
     if (weight_dtype == GTMOE_DTYPE_F32)
-        return wide ? forward_vec<__nv_bfloat16, float, float, 8>(a, st)
-                    : forward_vec<__nv_bfloat16, float, float, 1>(a, st);
-    return wide ? forward_vec<__nv_bfloat16, __nv_bfloat16, float, 8>(a, st)
-                : forward_vec<__nv_bfloat16, __nv_bfloat16, float, 1>(a, st);
+        return wide ? forward_vec<__nv_bfloat16, float, float, 8>(a, scope.device(), st)
+                    : forward_vec<__nv_bfloat16, float, float, 1>(a, scope.device(), st);
+    return wide ? forward_vec<__nv_bfloat16, __nv_bfloat16, float, 8>(a, scope.device(), st)
+                : forward_vec<__nv_bfloat16, __nv_bfloat16, float, 1>(a, scope.device(), st);
 }
 
 int gtmoe_layer_norm_workspace(int dtype, int64_t rows, int64_t width, int64_t *bytes) {
@@ -533,16 +856,16 @@ int gtmoe_layer_norm_backward(const void *dy, const void *x, int dtype, int64_t 
     const bool wide = width % vec == 0 && aligned16(x) && aligned16(dy) && aligned16(dresidual) && aligned16(dx) &&
                       aligned16(weight);
     if (dtype == GTMOE_DTYPE_F64)
-        return wide ? backward_vec<double, double, double, 2>(a, dweight, dbias, accumulate, st)
-                    : backward_vec<double, double, double, 1>(a, dweight, dbias, accumulate, st);
+        return wide ? backward_vec<double, double, double, 2>(a, dweight, dbias, accumulate, scope.device(), st)
+                    : backward_vec<double, double, double, 1>(a, dweight, dbias, accumulate, scope.device(), st);
     if (dtype == GTMOE_DTYPE_F32)
-        return wide ? backward_vec<float, float, float, 4>(a, dweight, dbias, accumulate, st)
-                    : backward_vec<float, float, float, 1>(a, dweight, dbias, accumulate, st);
+        return wide ? backward_vec<float, float, float, 4>(a, dweight, dbias, accumulate, scope.device(), st)
+                    : backward_vec<float, float, float, 1>(a, dweight, dbias, accumulate, scope.device(), st);
     if (weight_dtype == GTMOE_DTYPE_F32)
-        return wide ? backward_vec<__nv_bfloat16, float, float, 8>(a, dweight, dbias, accumulate, st)
-                    : backward_vec<__nv_bfloat16, float, float, 1>(a, dweight, dbias, accumulate, st);
-    return wide ? backward_vec<__nv_bfloat16, __nv_bfloat16, float, 8>(a, dweight, dbias, accumulate, st)
-                : backward_vec<__nv_bfloat16, __nv_bfloat16, float, 1>(a, dweight, dbias, accumulate, st);
+        return wide ? backward_vec<__nv_bfloat16, float, float, 8>(a, dweight, dbias, accumulate, scope.device(), st)
+                    : backward_vec<__nv_bfloat16, float, float, 1>(a, dweight, dbias, accumulate, scope.device(), st);
+    return wide ? backward_vec<__nv_bfloat16, __nv_bfloat16, float, 8>(a, dweight, dbias, accumulate, scope.device(), st)
+                : backward_vec<__nv_bfloat16, __nv_bfloat16, float, 1>(a, dweight, dbias, accumulate, scope.device(), st);
 }
 
 }  // extern "C"

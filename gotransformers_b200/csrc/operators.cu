@@ -74,9 +74,12 @@ extern "C" int gtmoe_operators_check(int device) {
     int before = 0, code = 0;
     GT_CUDA(cudaGetDevice(&before));
     GT_CUDA(cudaSetDevice(device));
-    const int rc = grouped_take_error(&code);
+    int norm = 0;
+    int rc = grouped_take_error(&code);
+    if (rc == 0) rc = norm_take_error(&norm);
     cudaSetDevice(before);
     GT_CHECK(rc);
+    if (norm != 0) return fail(GTMOE_ETIMEOUT, "layer norm: a kernel gave up waiting (barrier %d); results are invalid", norm);
     if (code == kErrBadCounts)
         return fail(GTMOE_EINVAL, "grouped product: a group had a negative count, or the counts' sum was above the rows; "
                                   "the call's results are invalid");

@@ -52,16 +52,51 @@ inline bool known_dtype(int t) { return t >= GTMOE_DTYPE_F64 && t <= GTMOE_DTYPE
 // rows x width elements of 8 bytes have to be countable in 63 bits
 inline bool countable(int64_t rows, int64_t width) { return width <= 0 || rows <= (INT64_MAX >> 4) / width; }
 
-// Bounded grouped-product waits and refused counts leave a code in a word of
-// the device (grouped_product.cu); gtmoe_operators_check reads it.
+// Bounded waits that ran out, and refused counts, leave a code in a word of the
+// device per source file; gtmoe_operators_check reads them.
 constexpr int kErrBadCounts = 101;
-// Waits for the current device, reads that word and clears it.
+// Each reads its words on the current device and clears them; the first waits
+// for the device.
 int grouped_take_error(int *code);
+int norm_take_error(int *code);
 
 // dropout.cu, for the block step (block.cu): device pointers, no checks.
 int check_dropout_rate(double rate);
 int launch_dropout(const void *x, const void *residual, int dtype, int64_t n, double rate, uint64_t seed,
                    uint64_t stream_id, int64_t offset, void *out, cudaStream_t st);
+
+// Two accumulators side by side: sm_100 multiplies and adds pairs of float32 in
+// one instruction.
+template <typename ACC>
+struct Pair {
+    ACC x, y;
+};
+__device__ __forceinline__ Pair<float> add2(Pair<float> a, Pair<float> b) {
+    const float2 r = __fadd2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y));
+    return {r.x, r.y};
+}
+__device__ __forceinline__ Pair<float> mul2(Pair<float> a, Pair<float> b) {
+    const float2 r = __fmul2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y));
+    return {r.x, r.y};
+}
+__device__ __forceinline__ Pair<float> fma2(Pair<float> a, Pair<float> b, Pair<float> c) {
+    const float2 r = __ffma2_rn(make_float2(a.x, a.y), make_float2(b.x, b.y), make_float2(c.x, c.y));
+    return {r.x, r.y};
+}
+__device__ __forceinline__ Pair<double> add2(Pair<double> a, Pair<double> b) { return {a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ Pair<double> mul2(Pair<double> a, Pair<double> b) { return {a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ Pair<double> fma2(Pair<double> a, Pair<double> b, Pair<double> c) {
+    return {fma(a.x, b.x, c.x), fma(a.y, b.y, c.y)};
+}
+template <typename ACC>
+__device__ __forceinline__ Pair<ACC> both(ACC v) {
+    return {v, v};
+}
+
+// Read-only data: the compiler may move these loads across stores.
+__device__ __forceinline__ uint4 load_const(const uint4 *p) { return __ldg(p); }
+__device__ __forceinline__ float4 load_const(const float4 *p) { return __ldg(p); }
+__device__ __forceinline__ double2 load_const(const double2 *p) { return __ldg(p); }
 
 // VEC consecutive values of T as ACC: one 16-byte access, or a plain one for VEC = 1.
 template <typename T, typename ACC, int VEC>
@@ -70,6 +105,9 @@ template <typename ACC>
 struct VecIO<__nv_bfloat16, ACC, 8> {
     using Raw = uint4;
     static __device__ __forceinline__ Raw load(const __nv_bfloat16 *p) { return *reinterpret_cast<const uint4 *>(p); }
+    static __device__ __forceinline__ Raw load_ro(const __nv_bfloat16 *p) {
+        return load_const(reinterpret_cast<const uint4 *>(p));
+    }
     static __device__ __forceinline__ void unpack(const Raw &r, ACC *v) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -92,6 +130,9 @@ template <>
 struct VecIO<float, float, 4> {
     using Raw = float4;
     static __device__ __forceinline__ Raw load(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+    static __device__ __forceinline__ Raw load_ro(const float *p) {
+        return load_const(reinterpret_cast<const float4 *>(p));
+    }
     static __device__ __forceinline__ void unpack(const Raw &r, float *v) {
         v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
     }
@@ -108,6 +149,9 @@ struct VecIO<float, float, 8> {
     static __device__ __forceinline__ Raw load(const float *p) {
         return {reinterpret_cast<const float4 *>(p)[0], reinterpret_cast<const float4 *>(p)[1]};
     }
+    static __device__ __forceinline__ Raw load_ro(const float *p) {
+        return {load_const(reinterpret_cast<const float4 *>(p)), load_const(reinterpret_cast<const float4 *>(p) + 1)};
+    }
     static __device__ __forceinline__ void unpack(const Raw &r, float *v) {
         v[0] = r.a.x, v[1] = r.a.y, v[2] = r.a.z, v[3] = r.a.w;
         v[4] = r.b.x, v[5] = r.b.y, v[6] = r.b.z, v[7] = r.b.w;
@@ -117,6 +161,9 @@ template <>
 struct VecIO<double, double, 2> {
     using Raw = double2;
     static __device__ __forceinline__ Raw load(const double *p) { return *reinterpret_cast<const double2 *>(p); }
+    static __device__ __forceinline__ Raw load_ro(const double *p) {
+        return load_const(reinterpret_cast<const double2 *>(p));
+    }
     static __device__ __forceinline__ void unpack(const Raw &r, double *v) { v[0] = r.x, v[1] = r.y; }
     static __device__ __forceinline__ void store(double *p, const double *v) {
         *reinterpret_cast<double2 *>(p) = make_double2(v[0], v[1]);

@@ -13,57 +13,80 @@ import ctypes
 from . import _lib
 from ._lib import DTYPE_BF16, DTYPE_F32, DTYPE_F64, check
 
+# torch, the library and the type codes, once an operator is first called
+# (importing this package needs neither)
+torch = None
+_L = None
 _CODES: dict = {}
 
 
-def _code(dtype) -> int:
-    if not _CODES:
-        import torch
+def _load():
+    global torch, _L
+    if torch is None:
+        import torch as torch_module
 
-        _CODES.update({torch.float64: DTYPE_F64, torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16})
+        _CODES.update({torch_module.float64: DTYPE_F64, torch_module.float32: DTYPE_F32,
+                       torch_module.bfloat16: DTYPE_BF16})
+        torch = torch_module
+    if _L is None:
+        _L = _lib.lib()
+
+
+def _code(dtype) -> int:
     code = _CODES.get(dtype)
     if code is None:
         raise ValueError(f"values must be float64, float32 or bfloat16, got {dtype}")
     return code
 
 
-def _tensor(name: str, a, shape=None, dtype=None, like=None):
-    """The checks every argument goes through; returns its address."""
+def _refuse(name: str, a, shape, dtype, device):
     if not hasattr(a, "data_ptr"):
         raise ValueError(f"{name} must be a CUDA tensor, got {type(a).__name__}")
     if not a.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device, got {a.device}")
     if not a.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if shape is not None and a.shape != shape:
+    if a.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(a.shape)}")
-    if dtype is not None and a.dtype != dtype:
+    if a.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {a.dtype}")
-    if like is not None and a.device != like.device:
-        raise ValueError(f"{name} is on {a.device} but the rows are on {like.device}")
-    return a.data_ptr()
+    raise ValueError(f"{name} is on {a.device} but the rows are on cuda:{device}")
 
 
-def _optional(name: str, a, shape=None, dtype=None, like=None):
-    return None if a is None else _tensor(name, a, shape, dtype, like)
-
-
-def _stream(a):
-    import torch
-
-    return torch.cuda.current_stream(a.device).cuda_stream
+def _tensor(name: str, a, shape, dtype, device: int):
+    """The checks an argument goes through; returns its address."""
+    try:
+        if (a.is_cuda and a.dtype is dtype and a.shape == shape and a.get_device() == device and a.is_contiguous()):
+            return a.data_ptr()
+    except AttributeError:
+        pass
+    return _refuse(name, a, shape, dtype, device)
 
 
 def _rows(name: str, a):
-    if getattr(a, "ndim", None) != 2:
-        raise ValueError(f"{name} must be rows x width, got {getattr(a, 'ndim', None)} dimensions")
-    return _tensor(name, a)
+    """The checks of the tensor that the others are held to; its address and device."""
+    address = _values(name, a)
+    if a.ndim != 2:
+        raise ValueError(f"{name} must be rows x width, got {a.ndim} dimensions")
+    return address
+
+
+def _values(name: str, a):
+    """_rows for a tensor of any shape."""
+    if torch is None or _L is None:
+        _load()
+    if not isinstance(a, torch.Tensor) or not a.is_cuda or not a.is_contiguous():
+        _refuse(name, a, getattr(a, "shape", None), getattr(a, "dtype", None), None)
+    return a.data_ptr(), a.get_device()
+
+
+def _stream(device: int) -> int:
+    """The device's current torch stream."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _stats_dtype(x):
-    import torch
-
-    return torch.float64 if x.dtype == torch.float64 else torch.float32
+    return torch.float64 if x.dtype is torch.float64 else torch.float32
 
 
 def layer_norm(x, weight=None, bias=None, epsilon: float = 1e-6, out=None):
@@ -71,21 +94,22 @@ def layer_norm(x, weight=None, bias=None, epsilon: float = 1e-6, out=None):
     weight and bias have x's dtype, or float32 beside bfloat16 rows.  Returns
     (y, mean, rstd); the statistics (float32, float64 for float64 rows) are
     what layer_norm_backward takes.  `out` may be x."""
-    import torch
-
-    px = _rows("x", x)
-    rows, width = x.shape
+    px, dev = _rows("x", x)
+    shape, dtype = x.shape, x.dtype
+    rows, width = shape
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"weight and bias must have one dtype, got {weight.dtype} and {bias.dtype}")
-    pw, pb = _optional("weight", weight, (width,), None, x), _optional("bias", bias, (width,), None, x)
-    wdt = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    wdt = weight.dtype if weight is not None else bias.dtype if bias is not None else dtype
+    pw = None if weight is None else _tensor("weight", weight, (width,), wdt, dev)
+    pb = None if bias is None else _tensor("bias", bias, (width,), wdt, dev)
+    code, wcode = _code(dtype), _code(wdt)
     if out is None:
         out = torch.empty_like(x)
-    po = _tensor("out", out, x.shape, x.dtype, x)
-    sdt = _stats_dtype(x)
-    mean, rstd = torch.empty(rows, dtype=sdt, device=x.device), torch.empty(rows, dtype=sdt, device=x.device)
-    check(_lib.lib().gtmoe_layer_norm(px, _code(x.dtype), rows, width, pw, pb, _code(wdt), epsilon, po,
-                                      mean.data_ptr(), rstd.data_ptr(), _stream(x)))
+    po = _tensor("out", out, shape, dtype, dev)
+    mean = torch.empty(rows, dtype=_stats_dtype(x), device=x.device)
+    rstd = torch.empty_like(mean)
+    check(_L.gtmoe_layer_norm(px, code, rows, width, pw, pb, wcode, epsilon, po, mean.data_ptr(), rstd.data_ptr(),
+                              _stream(dev)))
     return out, mean, rstd
 
 
@@ -98,36 +122,41 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
     weight's dtype (without a weight: float32, float64 for float64 rows) are
     returned, or None with want_parameters=False.  `input_gradients` may be
     any of the rows x width inputs."""
-    import torch
-
     g = output_gradients
-    pg = _rows("output_gradients", g)
-    rows, width = g.shape
-    px = _tensor("x", x, g.shape, g.dtype, g)
+    pg, dev = _rows("output_gradients", g)
+    shape, dtype = g.shape, g.dtype
+    rows, width = shape
+    code = _code(dtype)
+    px = _tensor("x", x, shape, dtype, dev)
     sdt = _stats_dtype(g)
-    pm, pr = _tensor("mean", mean, (rows,), sdt, g), _tensor("rstd", rstd, (rows,), sdt, g)
-    pw = _optional("weight", weight, (width,), None, g)
-    pres = _optional("residual_gradients", residual_gradients, g.shape, g.dtype, g)
-    wdt = weight.dtype if weight is not None else sdt
+    pm, pr = _tensor("mean", mean, (rows,), sdt, dev), _tensor("rstd", rstd, (rows,), sdt, dev)
+    wdt = weight.dtype if weight is not None else weight_grad.dtype if weight_grad is not None else sdt
+    wcode = _code(wdt)
+    pw = None if weight is None else _tensor("weight", weight, (width,), wdt, dev)
+    pres = None
+    if residual_gradients is not None:
+        pres = _tensor("residual_gradients", residual_gradients, shape, dtype, dev)
     if input_gradients is None:
         input_gradients = torch.empty_like(g)
-    pdx = _tensor("input_gradients", input_gradients, g.shape, g.dtype, g)
+    pdx = _tensor("input_gradients", input_gradients, shape, dtype, dev)
     if (weight_grad is None) != (bias_grad is None):
         raise ValueError("weight_grad and bias_grad are given together")
     accumulate = weight_grad is not None
-    pdw = pdb = work = None
-    nbytes = ctypes.c_int64(0)
+    pdw = pdb = pwork = None
+    nbytes = 0
     if accumulate or want_parameters:
         if not accumulate:
             weight_grad = torch.empty(width, dtype=wdt, device=g.device)
-            bias_grad = torch.empty(width, dtype=wdt, device=g.device)
-        pdw = _tensor("weight_grad", weight_grad, (width,), wdt, g)
-        pdb = _tensor("bias_grad", bias_grad, (width,), wdt, g)
-        check(_lib.lib().gtmoe_layer_norm_workspace(_code(g.dtype), rows, width, ctypes.byref(nbytes)))
-        work = torch.empty(nbytes.value, dtype=torch.uint8, device=g.device)
-    check(_lib.lib().gtmoe_layer_norm_backward(pg, px, _code(g.dtype), rows, width, pw, _code(wdt), pm, pr, pres, pdx,
-                                               pdw, pdb, int(accumulate), work.data_ptr() if work is not None else None,
-                                               nbytes.value, _stream(g)))
+            bias_grad = torch.empty_like(weight_grad)
+        pdw = _tensor("weight_grad", weight_grad, (width,), wdt, dev)
+        pdb = _tensor("bias_grad", bias_grad, (width,), wdt, dev)
+        need = ctypes.c_int64(0)
+        check(_L.gtmoe_layer_norm_workspace(code, rows, width, ctypes.byref(need)))
+        nbytes = need.value
+        work = torch.empty(nbytes, dtype=torch.uint8, device=g.device)
+        pwork = work.data_ptr()
+    check(_L.gtmoe_layer_norm_backward(pg, px, code, rows, width, pw, wcode, pm, pr, pres, pdx, pdw, pdb,
+                                       int(accumulate), pwork, nbytes, _stream(dev)))
     return input_gradients, weight_grad, bias_grad
 
 
@@ -136,14 +165,14 @@ def dropout(x, rate: float, seed: int, stream: int = 0, offset: int = 0, residua
     element i (in memory order) is kept depends on (seed, stream, offset + i)
     alone, so dropout_backward makes the same decisions again.  `out` may be
     x or residual."""
-    import torch
-
-    px = _tensor("x", x)
-    pr = _optional("residual", residual, x.shape, x.dtype, x)
+    px, dev = _values("x", x)
+    shape, dtype = x.shape, x.dtype
+    pr = None if residual is None else _tensor("residual", residual, shape, dtype, dev)
+    code = _code(dtype)
     if out is None:
         out = torch.empty_like(x)
-    po = _tensor("out", out, x.shape, x.dtype, x)
-    check(_lib.lib().gtmoe_dropout(px, pr, _code(x.dtype), x.numel(), rate, seed, stream, offset, po, _stream(x)))
+    po = _tensor("out", out, shape, dtype, dev)
+    check(_L.gtmoe_dropout(px, pr, code, x.numel(), rate, seed, stream, offset, po, _stream(dev)))
     return out
 
 
@@ -152,30 +181,23 @@ def dropout_backward(output_gradients, rate: float, seed: int, stream: int = 0, 
     """output_gradients * keep / (1 - rate), with dropout's decisions; the
     residual's gradients are the output gradients.  `input_gradients` may be
     output_gradients."""
-    import torch
-
     g = output_gradients
-    pg = _tensor("output_gradients", g)
+    pg, dev = _values("output_gradients", g)
+    code = _code(g.dtype)
     if input_gradients is None:
         input_gradients = torch.empty_like(g)
-    pdx = _tensor("input_gradients", input_gradients, g.shape, g.dtype, g)
-    check(_lib.lib().gtmoe_dropout_backward(pg, _code(g.dtype), g.numel(), rate, seed, stream, offset, pdx,
-                                            _stream(g)))
+    pdx = _tensor("input_gradients", input_gradients, g.shape, g.dtype, dev)
+    check(_L.gtmoe_dropout_backward(pg, code, g.numel(), rate, seed, stream, offset, pdx, _stream(dev)))
     return input_gradients
 
 
-def _weights(weights, like, like_name: str, axis: int):
-    pw = _tensor("weights", weights, None, like.dtype, like)
-    if weights.ndim != 3 or weights.shape[axis] != like.shape[1]:
+def _weights(weights, like, like_name: str, axis: int, dev: int):
+    """The weights' address, groups, outputs and inputs."""
+    shape = getattr(weights, "shape", ())
+    if len(shape) != 3 or shape[axis] != like.shape[1]:
         raise ValueError(f"weights must be groups x outputs x inputs and fit {like_name}'s {like.shape[1]} columns, "
-                         f"got {tuple(weights.shape)}")
-    return pw
-
-
-def _counts(counts, groups, like):
-    import torch
-
-    return _tensor("counts", counts, (groups,), torch.int64, like)
+                         f"got {tuple(shape)}")
+    return _tensor("weights", weights, shape, like.dtype, dev), *shape
 
 
 def grouped_product(x, weights, counts, out=None):
@@ -183,35 +205,30 @@ def grouped_product(x, weights, counts, out=None):
     holds counts[0] rows of group 0, then counts[1] of group 1, ... (counts an
     int64 CUDA tensor); weights are groups x outputs x inputs.  Rows after the
     last group's are not written."""
-    import torch
-
-    px = _rows("x", x)
-    pw = _weights(weights, x, "x", 2)
-    groups, outputs, inputs = weights.shape
-    rows = x.shape[0]
-    pc = _counts(counts, groups, x)
+    px, dev = _rows("x", x)
+    pw, groups, outputs, inputs = _weights(weights, x, "x", 2, dev)
+    rows, dtype = x.shape[0], x.dtype
+    pc = _tensor("counts", counts, (groups,), torch.int64, dev)
+    code = _code(dtype)
     if out is None:
-        out = torch.empty((rows, outputs), dtype=x.dtype, device=x.device)
-    po = _tensor("out", out, (rows, outputs), x.dtype, x)
-    check(_lib.lib().gtmoe_grouped_product(px, pw, _code(x.dtype), rows, inputs, outputs, groups, pc, po, _stream(x)))
+        out = torch.empty((rows, outputs), dtype=dtype, device=x.device)
+    po = _tensor("out", out, (rows, outputs), dtype, dev)
+    check(_L.gtmoe_grouped_product(px, pw, code, rows, inputs, outputs, groups, pc, po, _stream(dev)))
     return out
 
 
 def grouped_product_input_gradients(output_gradients, weights, counts, input_gradients=None):
     """output_gradients[r] @ weights[g] for the rows r of each group g."""
-    import torch
-
     g = output_gradients
-    pg = _rows("output_gradients", g)
-    pw = _weights(weights, g, "output_gradients", 1)
-    groups, outputs, inputs = weights.shape
-    rows = g.shape[0]
-    pc = _counts(counts, groups, g)
+    pg, dev = _rows("output_gradients", g)
+    pw, groups, outputs, inputs = _weights(weights, g, "output_gradients", 1, dev)
+    rows, dtype = g.shape[0], g.dtype
+    pc = _tensor("counts", counts, (groups,), torch.int64, dev)
+    code = _code(dtype)
     if input_gradients is None:
-        input_gradients = torch.empty((rows, inputs), dtype=g.dtype, device=g.device)
-    pdx = _tensor("input_gradients", input_gradients, (rows, inputs), g.dtype, g)
-    check(_lib.lib().gtmoe_grouped_product_input_grad(pg, pw, _code(g.dtype), rows, inputs, outputs, groups, pc, pdx,
-                                                      _stream(g)))
+        input_gradients = torch.empty((rows, inputs), dtype=dtype, device=g.device)
+    pdx = _tensor("input_gradients", input_gradients, (rows, inputs), dtype, dev)
+    check(_L.gtmoe_grouped_product_input_grad(pg, pw, code, rows, inputs, outputs, groups, pc, pdx, _stream(dev)))
     return input_gradients
 
 
@@ -219,39 +236,36 @@ def grouped_product_weight_gradients(output_gradients, x, counts, weight_grad=No
     """The sum over group g's rows of output_gradients[r].T @ x[r], groups x
     outputs x inputs.  weight_grad, where given, has them added; else a new
     tensor of `dtype` (x's dtype, or float32 beside bfloat16) is returned."""
-    import torch
-
     g = output_gradients
-    pg = _rows("output_gradients", g)
-    px = _rows("x", x)
-    _tensor("x", x, None, g.dtype, g)
-    if x.shape[0] != g.shape[0]:
-        raise ValueError(f"x has {x.shape[0]} rows but output_gradients {g.shape[0]}")
-    rows, outputs, inputs = g.shape[0], g.shape[1], x.shape[1]
+    pg, dev = _rows("output_gradients", g)
+    px, _ = _rows("x", x)
+    rows, outputs = g.shape
+    inputs = x.shape[1]
+    _tensor("x", x, (rows, inputs), g.dtype, dev)
     if getattr(counts, "ndim", None) != 1:
         raise ValueError("counts must be one number per group")
     groups = counts.shape[0]
-    pc = _counts(counts, groups, g)
+    pc = _tensor("counts", counts, (groups,), torch.int64, dev)
+    code = _code(g.dtype)
     accumulate = weight_grad is not None
     if not accumulate:
         weight_grad = torch.empty((groups, outputs, inputs), dtype=dtype or g.dtype, device=g.device)
     elif dtype is not None and weight_grad.dtype != dtype:
         raise ValueError(f"weight_grad is {weight_grad.dtype} but dtype {dtype}")
-    pdw = _tensor("weight_grad", weight_grad, (groups, outputs, inputs), None, g)
-    nbytes, work = ctypes.c_int64(0), None
-    check(_lib.lib().gtmoe_grouped_product_workspace(_code(g.dtype), rows, inputs, outputs, groups,
-                                                     ctypes.byref(nbytes)))
-    if nbytes.value:
-        work = torch.empty(nbytes.value, dtype=torch.uint8, device=g.device)
-    check(_lib.lib().gtmoe_grouped_product_weight_grad(pg, px, _code(g.dtype), rows, inputs, outputs, groups, pc, pdw,
-                                                       _code(weight_grad.dtype), int(accumulate),
-                                                       work.data_ptr() if work is not None else None, nbytes.value,
-                                                       _stream(g)))
+    wcode = _code(weight_grad.dtype)
+    pdw = _tensor("weight_grad", weight_grad, (groups, outputs, inputs), weight_grad.dtype, dev)
+    need, pwork = ctypes.c_int64(0), None
+    check(_L.gtmoe_grouped_product_workspace(code, rows, inputs, outputs, groups, ctypes.byref(need)))
+    if need.value:
+        work = torch.empty(need.value, dtype=torch.uint8, device=g.device)
+        pwork = work.data_ptr()
+    check(_L.gtmoe_grouped_product_weight_grad(pg, px, code, rows, inputs, outputs, groups, pc, pdw, wcode,
+                                               int(accumulate), pwork, need.value, _stream(dev)))
     return weight_grad
 
 
 def check_operators(device: int = 0):
-    """Waits for the device and raises GtmoeError if a grouped product since
-    the last check was given impossible counts (EINVAL) or gave up waiting
+    """Waits for the device and raises GtmoeError if an operator since the
+    last check was given impossible counts (EINVAL) or gave up waiting
     (ETIMEOUT)."""
     check(_lib.lib().gtmoe_operators_check(device))

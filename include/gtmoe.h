@@ -386,8 +386,7 @@ GTMOE_API int gtmoe_grouped_product_weight_grad(const void *dy, const void *x, i
                                       int dw_dtype, int accumulate, void *workspace, int64_t workspace_bytes,
                                       void *stream);
 
-/* What the grouped products' kernels recorded on `device` since the last
- * check: waits for the device, then 0, GTMOE_EINVAL (refused counts) or
+/* What the operators' kernels recorded on `device` since the last check: waits for the device, then 0, GTMOE_EINVAL (refused counts) or
  * GTMOE_ETIMEOUT (a bounded wait ran out); the record is cleared.  Not inside
  * a stream capture. */
 GTMOE_API int gtmoe_operators_check(int device);

@@ -2,7 +2,7 @@
 
 Tolerances: an output is rounded once (HALF of its type, relative), after sums
 in the type's UNIT.  A thread adds at most 64 values of a row (width / 256 of
-a row too wide for registers), then at most 5 + 16 steps join the threads, and
+a row too wide for shared memory), then at most 5 + 16 steps join the threads, and
 the mean, the variance and each product round a few times more: ADDS additions
 in a row bound the relative error of every sum.  The mean's error enters xh
 divided by the deviation, so AMP = 1 + max|x| rstd multiplies it."""
@@ -64,7 +64,7 @@ def check_backward(x, w, dy, dres, eps, got_dx, got_dw, got_db, wdtype, before=N
     R.within("dx", got_dx, dx, R.HALF[x.dtype] * dx.abs() + bound[:, None] * (1 + R.HALF[x.dtype])
              + (u * dx.abs() if dres is not None else 0))
     rows = x.shape[0]
-    # rows in a row within one team, then teams, runs of partial rows and the runs' sum
+    # rows in a row within one team, then teams, runs of partial rows and the runs' sum (fewer than these)
     chain = rows / 296 + 1 + 16 + 296 / 16 + 16 + 4
     tw = u * (chain * (dy.double() * xh).abs().sum(0) + a * (dy.double().abs() * amp[:, None]).sum(0))
     tb = u * chain * dy.double().abs().sum(0)
