@@ -9,24 +9,67 @@ namespace {
 
 __device__ int g_error;  // first code a kernel recorded since the last check
 
-constexpr int kTile = 64;   // rows and columns of a block's tile
 constexpr int kStep = 16;   // terms of the sums per shared-memory step
 constexpr int kThreads = 256;
+
+// One operand of a tile: `n` values along the tile's axis by kStep terms.
+// KMAJOR: the terms are contiguous in memory, else the tile's axis is.
+// Consecutive threads load along the contiguous axis, into registers while the
+// step before is multiplied, then into shared memory as [term][value].
+template <typename T, typename ACC, int TILE, bool KMAJOR>
+struct Operand {
+    static constexpr int kLoads = TILE * kStep / kThreads;
+    const T *p;      // this thread's first value of step 0
+    int64_t q_step, k_step;
+    int at, term;    // its place in the tile
+    int64_t n, terms;
+    ACC v[kLoads];
+
+    // base: value 0, term 0; ld: distance of the outer axis
+    __device__ __forceinline__ void begin(const T *base, int64_t ld, int64_t n_values, int64_t n_terms) {
+        const int t = threadIdx.x;
+        term = KMAJOR ? t % kStep : t / TILE;
+        at = KMAJOR ? t / kStep : t % TILE;
+        p = base + (KMAJOR ? at * ld + term : term * ld + at);
+        q_step = (KMAJOR ? kThreads / kStep : kThreads / TILE) * ld;
+        k_step = KMAJOR ? kStep : kStep * ld;
+        n = n_values;
+        terms = n_terms;
+    }
+    __device__ __forceinline__ void load(int64_t k0) {
+#pragma unroll
+        for (int q = 0; q < kLoads; q++) {
+            const int i = KMAJOR ? at + q * (kThreads / kStep) : at;
+            const int64_t k = k0 + (KMAJOR ? term : term + q * (kThreads / TILE));
+            v[q] = i < n && k < terms ? (ACC)p[q * q_step] : ACC(0);
+        }
+        p += k_step;
+    }
+    __device__ __forceinline__ void store(ACC (*s)[TILE + 4]) const {
+#pragma unroll
+        for (int q = 0; q < kLoads; q++) {
+            if (KMAJOR) s[term][at + q * (kThreads / kStep)] = v[q];
+            else s[term + q * (kThreads / TILE)][at] = v[q];
+        }
+    }
+};
 
 // C[i][j] = sum over p of A(i, p) B(j, p):
 //   kProduct     i row, j output, p input:   A = X[i][p],  B = W_g[j][p]
 //   kInputGrad   i row, j input,  p output:  A = dY[i][p], B = W_g[p][j]
 //   kWeightGrad  i output, j input, p row:   A = dY[p][i], B = X[p][j]
-// 4 x 4 outputs per thread, each one sum in ascending p in ACC.
-template <typename T, typename ACC, typename OUT, GroupedOp OP>
+// TILE x TILE outputs per block, (TILE / 16)^2 per thread, each one sum in
+// ascending p in ACC.  Two buffers: one barrier per step.
+template <typename T, typename ACC, typename OUT, GroupedOp OP, int TILE>
 __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const GroupedProduct a) {
-    __shared__ ACC sa[kStep][kTile + 4], sb[kStep][kTile + 4];
+    constexpr int R = TILE / 16, V = R < 4 ? R : 4;  // outputs per thread and axis, in runs of V
+    __shared__ __align__(16) ACC sa[2][kStep][TILE + 4], sb[2][kStep][TILE + 4];
     __shared__ int start[kMaxGroups + 1], tiles[kMaxGroups + 1], scratch[kThreads];
     const int64_t n_j = OP == kProduct ? a.outputs : a.inputs;
-    const int64_t j_tiles = (n_j + kTile - 1) / kTile;
+    const int64_t j_tiles = (n_j + TILE - 1) / TILE;
     const bool ok = OP == kWeightGrad ? group_ranges(a.counts, a.groups, a.rows, kAnyRows, 1,
-                                                     (int)((a.outputs + kTile - 1) / kTile), start, tiles, scratch)
-                                      : group_ranges(a.counts, a.groups, a.rows, kTile, 0, 1, start, tiles, scratch);
+                                                     (int)((a.outputs + TILE - 1) / TILE), start, tiles, scratch)
+                                      : group_ranges(a.counts, a.groups, a.rows, TILE, 0, 1, start, tiles, scratch);
     if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_error, 0, kErrBadCounts);
     const int64_t total = (int64_t)tiles[a.groups] * j_tiles;
     const T *A = (const T *)a.a, *B = (const T *)a.b;
@@ -35,53 +78,54 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
     for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
         const int it = (int)(u / j_tiles);
         while (tiles[g + 1] <= it) g++;
-        const int64_t i0 = (int64_t)(it - tiles[g]) * kTile, j0 = (u % j_tiles) * kTile;
+        const int64_t i0 = (int64_t)(it - tiles[g]) * TILE, j0 = (u % j_tiles) * TILE;
         const int64_t r0 = start[g], m = start[g + 1] - start[g];
         const int64_t i_end = OP == kWeightGrad ? a.outputs : m;
         const int64_t p_end = OP == kProduct ? a.inputs : OP == kInputGrad ? a.outputs : m;
         const T *Wg = B + (int64_t)g * a.outputs * a.inputs;
-        ACC acc[4][4] = {};
-        for (int64_t p0 = 0; p0 < p_end; p0 += kStep) {
-            // consecutive threads along the operand's contiguous axis
-#pragma unroll
-            for (int q = 0; q < kTile * kStep / kThreads; q++) {
-                const int e = q * kThreads + threadIdx.x;
-                const int ap = OP == kWeightGrad ? e / kTile : e % kStep, ai = OP == kWeightGrad ? e % kTile : e / kStep;
-                const int bp = OP == kProduct ? e % kStep : e / kTile, bj = OP == kProduct ? e / kStep : e % kTile;
-                ACC va = ACC(0), vb = ACC(0);
-                if (i0 + ai < i_end && p0 + ap < p_end)
-                    va = (ACC)(OP == kWeightGrad ? A[(r0 + p0 + ap) * a.outputs + i0 + ai]
-                                                 : A[(r0 + i0 + ai) * (OP == kProduct ? a.inputs : a.outputs) + p0 + ap]);
-                if (j0 + bj < n_j && p0 + bp < p_end)
-                    vb = (ACC)(OP == kProduct      ? Wg[(j0 + bj) * a.inputs + p0 + bp]
-                               : OP == kInputGrad ? Wg[(p0 + bp) * a.inputs + j0 + bj]
-                                                  : B[(r0 + p0 + bp) * a.inputs + j0 + bj]);
-                sa[ap][ai] = va;
-                sb[bp][bj] = vb;
+        Operand<T, ACC, TILE, OP != kWeightGrad> oa;
+        Operand<T, ACC, TILE, OP == kProduct> ob;
+        if (OP == kWeightGrad) oa.begin(A + r0 * a.outputs + i0, a.outputs, i_end - i0, p_end);
+        else oa.begin(A + (r0 + i0) * p_end, p_end, i_end - i0, p_end);
+        if (OP == kProduct) ob.begin(Wg + j0 * a.inputs, a.inputs, n_j - j0, p_end);
+        else if (OP == kInputGrad) ob.begin(Wg + j0, a.inputs, n_j - j0, p_end);
+        else ob.begin(B + r0 * a.inputs + j0, a.inputs, n_j - j0, p_end);
+        ACC acc[R][R] = {};
+        oa.load(0);
+        ob.load(0);
+        int buf = 0;
+        for (int64_t p0 = 0; p0 < p_end; p0 += kStep, buf ^= 1) {
+            oa.store(sa[buf]);
+            ob.store(sb[buf]);
+            __syncthreads();  // also: the step before last has been multiplied by every thread
+            if (p0 + kStep < p_end) {
+                oa.load(p0 + kStep);
+                ob.load(p0 + kStep);
             }
-            __syncthreads();
 #pragma unroll
             for (int p = 0; p < kStep; p++) {
-                ACC ra[4], rb[4];
+                ACC ra[R], rb[R];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    ra[q] = sa[p][ty * 4 + q];
-                    rb[q] = sb[p][tx * 4 + q];
-                }
+                for (int h = 0; h < R / V; h++)
 #pragma unroll
-                for (int x = 0; x < 4; x++)
+                    for (int q = 0; q < V; q++) {
+                        ra[h * V + q] = sa[buf][p][h * 16 * V + ty * V + q];
+                        rb[h * V + q] = sb[buf][p][h * 16 * V + tx * V + q];
+                    }
 #pragma unroll
-                    for (int y = 0; y < 4; y++) acc[x][y] += ra[x] * rb[y];
+                for (int x = 0; x < R; x++)
+#pragma unroll
+                    for (int y = 0; y < R; y++) acc[x][y] += ra[x] * rb[y];
             }
-            __syncthreads();
         }
+        __syncthreads();  // the buffers are free for the next tile
         OUT *C = (OUT *)a.c;
         const int64_t base = OP == kWeightGrad ? (int64_t)g * a.outputs * a.inputs : r0 * n_j;
 #pragma unroll
-        for (int x = 0; x < 4; x++)
+        for (int x = 0; x < R; x++)
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const int64_t i = i0 + ty * 4 + x, j = j0 + tx * 4 + y;
+            for (int y = 0; y < R; y++) {
+                const int64_t i = i0 + x / V * 16 * V + ty * V + x % V, j = j0 + y / V * 16 * V + tx * V + y % V;
                 if (i < i_end && j < n_j) {
                     OUT &o = C[base + i * n_j + j];
                     o = (OUT)(OP == kWeightGrad && a.accumulate ? (ACC)o + acc[x][y] : acc[x][y]);
@@ -90,18 +134,34 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
     }
 }
 
-template <typename T, typename ACC, typename OUT, GroupedOp OP>
-int launch_simt(const GroupedProduct &p, cudaStream_t st) {
+template <typename T, typename ACC, typename OUT, GroupedOp OP, int TILE>
+int launch_simt_tile(const GroupedProduct &p, int64_t *tiles, cudaStream_t st) {
     const int64_t n_j = OP == kProduct ? p.outputs : p.inputs;
     // at most this many tiles: the rows of a group end inside a tile
-    const int64_t i_tiles = OP == kWeightGrad ? (int64_t)p.groups * ((p.outputs + kTile - 1) / kTile)
-                                              : p.rows / kTile + (p.rows < p.groups ? p.rows : p.groups);
-    const int64_t most = i_tiles * ((n_j + kTile - 1) / kTile);
+    const int64_t i_tiles = OP == kWeightGrad ? (int64_t)p.groups * ((p.outputs + TILE - 1) / TILE)
+                                              : p.rows / TILE + (p.rows < p.groups ? p.rows : p.groups);
+    const int64_t most = i_tiles * ((n_j + TILE - 1) / TILE);
+    if (tiles) {
+        *tiles = most;
+        return 0;
+    }
     const unsigned grid = (unsigned)(most < 148 * 16 ? most : 148 * 16);
-    grouped_simt_product_kernel<T, ACC, OUT, OP><<<grid, kThreads, 0, st>>>(p);
+    grouped_simt_product_kernel<T, ACC, OUT, OP, TILE><<<grid, kThreads, 0, st>>>(p);
     GT_CUDA(cudaGetLastError());
     note_launches(1);
     return 0;
+}
+
+// Tiles of 128 x 128 (64 products per 16 values read) once they are enough for
+// every SM, else of 64 x 64; float64 has shared memory for the latter only.
+template <typename T, typename ACC, typename OUT, GroupedOp OP>
+int launch_simt(const GroupedProduct &p, cudaStream_t st) {
+    if constexpr (sizeof(ACC) == 4) {
+        int64_t tiles = 0;
+        GT_CHECK((launch_simt_tile<T, ACC, OUT, OP, 128>(p, &tiles, st)));
+        if (tiles >= 2 * 148) return launch_simt_tile<T, ACC, OUT, OP, 128>(p, nullptr, st);
+    }
+    return launch_simt_tile<T, ACC, OUT, OP, 64>(p, nullptr, st);
 }
 
 template <typename T, typename ACC>
@@ -125,7 +185,7 @@ int check_sizes(const GroupedProduct &p) {
         return fail(GTMOE_EINVAL, "grouped product: needs 1 to %d groups, got %d", kMaxGroups, p.groups);
     if (!countable(p.rows, p.inputs) || !countable(p.rows, p.outputs) || !countable(p.inputs * p.groups, p.outputs))
         return fail(GTMOE_EINVAL, "grouped product: an operand is too large");
-    if ((p.outputs + kTile - 1) / kTile * p.groups > 0x7fffffff)
+    if ((p.outputs + 63) / 64 * p.groups > 0x7fffffff)
         return fail(GTMOE_EINVAL, "grouped product: too many outputs for %d groups", p.groups);
     return 0;
 }
