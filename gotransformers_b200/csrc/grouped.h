@@ -31,29 +31,38 @@ struct GroupedProduct {
 constexpr int kMaxGroups = kMaxRoutedExperts;
 constexpr int kAnyRows = 0x7fffffff;  // a tile_rows that no group fills
 
-// Inclusive scan of one value per thread of the block over the threads, cut at
-// `most` (< 2^31; cutting a sum of non-negative values early or late gives the
-// same).  `scratch` is one word per thread; returns the threads' sum before
-// this one's.
+// The sum of the threads' values before this one's, cut at `most` (< 2^31;
+// cutting a sum of non-negative values early or late gives the same).  Every
+// thread of the block calls it; `scratch` is one word per warp, free again when
+// it returns.
 __device__ __forceinline__ int64_t block_scan(int64_t own, int64_t most, int *scratch) {
-    const int t = threadIdx.x;
-    scratch[t] = (int)(own < most ? own : most);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    auto cut = [&](int64_t v) { return (int)(v < most ? v : most); };
+    auto warp_scan = [&](int v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v = cut((int64_t)v + u);
+        }
+        return v;
+    };
+    const int sum = warp_scan(cut(own));
+    if (lane == 31) scratch[warp] = sum;
     __syncthreads();
-    for (int o = 1; o < (int)blockDim.x; o <<= 1) {
-        const int64_t v = (int64_t)scratch[t] + (t >= o ? scratch[t - o] : 0);
-        __syncthreads();
-        scratch[t] = (int)(v < most ? v : most);
-        __syncthreads();
-    }
-    return t ? scratch[t - 1] : 0;
+    // every warp scans the warps' sums for itself
+    const int all = warp_scan(lane < warps ? scratch[lane] : 0);
+    const int before = __shfl_sync(0xffffffffu, all, (warp + 31) & 31);
+    const int mine = __shfl_up_sync(0xffffffffu, sum, 1);
+    __syncthreads();
+    return cut((int64_t)(warp ? before : 0) + (lane ? mine : 0));
 }
 
 // Group g's rows are start[g] .. start[g + 1], cut at `rows`; a negative
 // count is no rows.  tiles[g] is the number of tiles before group g: `per` for
 // each run of tile_rows rows that it has begun, of which it has at least
 // `least`.  Every thread of the block calls it; start and tiles are groups + 1
-// words of shared memory, scratch one word per thread.  True when the counts
-// were as they should be.
+// words of shared memory, scratch one word per warp.  True when the counts were
+// as they should be.
 __device__ __forceinline__ bool group_ranges(const int64_t *__restrict__ counts, int groups, int64_t rows,
                                              int tile_rows, int least, int per, int *start, int *tiles,
                                              int *scratch) {
@@ -83,7 +92,6 @@ __device__ __forceinline__ bool group_ranges(const int64_t *__restrict__ counts,
         n_tiles += n;
         tiles[g + 1] = (int)n;
     }
-    __syncthreads();
     at = block_scan(n_tiles, 0x7ffffffe, scratch);
     for (int g = g0; g < g1; g++) {
         at += tiles[g + 1];

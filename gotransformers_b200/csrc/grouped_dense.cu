@@ -73,7 +73,7 @@ constexpr int kGradPitch = 36;
 constexpr int kEpiBytes = kEpiWarps * 32 * kGradPitch * 4;
 static_assert(4 * kRowBuf <= kEpiBytes, "epilogue staging");
 constexpr int kBarBytes = 256;
-constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiBytes + kBarBytes + (2 * (kMaxGroups + 1) + kThreads) * 4;
+constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiBytes + kBarBytes + (2 * (kMaxGroups + 1) + kThreads / 32) * 4;
 static_assert(kSmemBytes <= 232448, "shared memory per CTA");
 
 struct DenseArgs {
@@ -679,7 +679,7 @@ int part_rows(int64_t rows, int64_t inputs, int64_t outputs, int groups) {
 // Adds the parts' sums of every group that was split, in order, four values
 // per thread.
 __global__ void __launch_bounds__(256) add_parts_kernel(const DenseArgs a) {
-    __shared__ int start[kMaxGroups + 1], first[kMaxGroups + 1], scratch[256];
+    __shared__ int start[kMaxGroups + 1], first[kMaxGroups + 1], scratch[8];
     group_ranges(a.counts, a.groups, a.rows, a.part_rows, 1, 1, start, first, scratch);
     const int64_t area = (int64_t)a.outputs * a.inputs;
     for (int g = 0; g < a.groups; g++) {

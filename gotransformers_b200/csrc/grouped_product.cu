@@ -64,7 +64,7 @@ template <typename T, typename ACC, typename OUT, GroupedOp OP, int TILE>
 __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const GroupedProduct a) {
     constexpr int R = TILE / 16, V = R < 4 ? R : 4;  // outputs per thread and axis, in runs of V
     __shared__ __align__(16) ACC sa[2][kStep][TILE + 4], sb[2][kStep][TILE + 4];
-    __shared__ int start[kMaxGroups + 1], tiles[kMaxGroups + 1], scratch[kThreads];
+    __shared__ int start[kMaxGroups + 1], tiles[kMaxGroups + 1], scratch[kThreads / 32];
     const int64_t n_j = OP == kProduct ? a.outputs : a.inputs;
     const int64_t j_tiles = (n_j + TILE - 1) / TILE;
     const bool ok = OP == kWeightGrad ? group_ranges(a.counts, a.groups, a.rows, kAnyRows, 1,
