@@ -641,7 +641,7 @@ struct View {
     int box[4];
 };
 int encode_view(CUtensorMap *map, const void *base, const View &v, bool f32 = false) {
-    auto enc = tensor_map_encoder();
+    static const auto enc = tensor_map_encoder();  // looked up once, whichever thread comes first
     if (!enc) return fail(GTMOE_ECUDA, "cuTensorMapEncodeTiled is not available");
     cuuint64_t dims[4], strides[3];
     cuuint32_t boxes[4], ones[4] = {1, 1, 1, 1};

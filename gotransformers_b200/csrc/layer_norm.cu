@@ -27,15 +27,15 @@ constexpr int kRingThreads = 256;
 constexpr int kBwdBlocks = 2 * 148;
 // A ring's mbarriers and abort flag come before its stages in shared memory.
 constexpr int kMaxStages = 8;
-constexpr int kRingHeader = 256;
+constexpr int kRingHeader = 512;
 // Shared memory for the stages of a backward's block of 256 threads (of 512:
 // twice this): two blocks per SM.
 constexpr int kBwdStageBytes = 98304;
-// The forward: warps per block, tiles in a warp's ring, and shared memory for
-// a block's rings.
-constexpr int kFwdMostWarps = 8;
-constexpr int kFwdStages = 2;
-constexpr int kFwdMostBytes = 200 * 1024;
+// The forward: most warps per block, most tiles in a warp's ring, and shared
+// memory for a block's rings and parameters.
+constexpr int kFwdMostWarps = 16;
+constexpr int kFwdStages = 3;
+constexpr int kFwdMostBytes = 224 * 1024;
 static_assert(2 * kMaxStages * 8 + 4 <= kRingHeader && kFwdMostWarps * (kFwdStages * 8 + 4) <= kRingHeader, "ring header");
 
 __device__ int g_norm_error;  // a bounded wait's code (gtmoe_operators_check)
@@ -85,7 +85,8 @@ struct NormArgs {
     int64_t rows;
     int width;
     double eps;
-    int team, stages;  // of the backward's ring
+    int team, stages;   // threads per row of the backward; tiles in a ring
+    int shared_params;  // bytes of the forward's copy of its parameters
     // backward
     const void *dy, *dres;
     void *dx;
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kFwdMostWarps * 32) norm_forward_kernel(const 
     const int64_t row_bytes = (int64_t)n * (int64_t)sizeof(T), tile_bytes = row_bytes * RP;
     uint64_t *full = (uint64_t *)smem + warp * kFwdStages;
     int *abort_flag = (int *)((uint64_t *)smem + kFwdMostWarps * kFwdStages) + warp;
-    uint8_t *data = smem + kRingHeader + warp * kFwdStages * tile_bytes;
+    uint8_t *data = smem + kRingHeader + a.shared_params + warp * a.stages * tile_bytes;
     const int64_t tiles = (a.rows + RP - 1) / RP, step = (int64_t)gridDim.x * warps;
     const int64_t first = (int64_t)blockIdx.x * warps + warp;
     auto fill = [&](int64_t t, int stage) {
@@ -230,14 +231,25 @@ __global__ void __launch_bounds__(kFwdMostWarps * 32) norm_forward_kernel(const 
             : "memory");
     };
     if (lane == 0) {
-        for (int s = 0; s < kFwdStages; s++) mbar_init(&full[s], 1);
+        for (int s = 0; s < a.stages; s++) mbar_init(&full[s], 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        for (int s = 0; s < kFwdStages; s++)
+        for (int s = 0; s < a.stages; s++)
             if (first + s * step < tiles) fill(first + s * step, s);
     }
     __syncwarp();
     const W *w = (const W *)a.weight, *b = (const W *)a.bias;
+    if (a.shared_params) {
+        // the rings leave L1 too small to keep the parameters: one copy for the block's warps
+        W *sw = (W *)(smem + kRingHeader), *sb = w ? sw + n : sw;
+        for (int c = threadIdx.x * VEC; c < n; c += blockDim.x * VEC) {
+            if (w) *reinterpret_cast<typename P::Raw *>(sw + c) = P::load_ro(w + c);
+            if (b) *reinterpret_cast<typename P::Raw *>(sb + c) = P::load_ro(b + c);
+        }
+        __syncthreads();
+        if (w) w = sw;
+        if (b) b = sb;
+    }
     int stage = 0;
     uint32_t phase = 0;
     for (int64_t t = first; t < tiles; t += step) {
@@ -290,8 +302,8 @@ __global__ void __launch_bounds__(kFwdMostWarps * 32) norm_forward_kernel(const 
 #pragma unroll 4
         for (int c = lane * VEC; c < n; c += 32 * VEC) {
             Pair<ACC> pw[H], pb[H];
-            if (w) P::unpack(P::load_ro(w + c), &pw[0].x);
-            if (b) P::unpack(P::load_ro(b + c), &pb[0].x);
+            if (w) P::unpack(P::load(w + c), &pw[0].x);
+            if (b) P::unpack(P::load(b + c), &pb[0].x);
 #pragma unroll
             for (int r = 0; r < RP; r++) {
                 X::unpack(X::load(x + r * n + c), &v[0].x);
@@ -314,8 +326,8 @@ __global__ void __launch_bounds__(kFwdMostWarps * 32) norm_forward_kernel(const 
             if (a.rstd) ((ACC *)a.rstd)[row + lane] = rs;
         }
         __syncwarp();  // the stage has been read
-        if (lane == 0 && t + kFwdStages * step < tiles) fill(t + kFwdStages * step, stage);
-        if (++stage == kFwdStages) {
+        if (lane == 0 && t + a.stages * step < tiles) fill(t + a.stages * step, stage);
+        if (++stage == a.stages) {
             stage = 0;
             phase ^= 1;
         }
@@ -659,20 +671,32 @@ int forward_vec(NormArgs a, int device, cudaStream_t st) {
         // rows per warp: tiles of up to 8 KB, as long as every SM's warps get one
         int rp = bytes <= 2048 ? 4 : bytes <= 4096 ? 2 : 1;
         while (rp > 1 && a.rows < (int64_t)rp * 148 * 12) rp /= 2;
-        // small tiles: blocks of four warps, three or more per SM; large ones: one block of what fits
-        const int64_t ring = bytes * rp * kFwdStages, fit = kFwdMostBytes / ring;
-        if (fit >= 2) {
+        // rows above 4 KB: one block per SM of as many warps as have room for rings of three tiles (two, where that
+        // leaves fewer than eight warps), the parameters beside them (65536 x 4096 bf16: 217 -> 201 us); shorter or few
+        // rows: blocks of four warps with rings of two, and L1 keeps the parameters
+        const int64_t tile = bytes * rp, tiles = (a.rows + rp - 1) / rp;
+        const int64_t params = ((a.weight ? 1 : 0) + (a.bias ? 1 : 0)) * (int64_t)a.width * sizeof(W);
+        int64_t stages = kFwdMostBytes - params >= 8 * 3 * tile ? 3 : 2, warps = (kFwdMostBytes - params) / (stages * tile);
+        if (warps > kFwdMostWarps) warps = kFwdMostWarps;
+        const bool share = bytes > 4096 && warps >= 2 && tiles >= 148 * 2 * warps;
+        if (!share) {
+            stages = 2;
+            warps = kFwdMostBytes / (stages * tile);
+            if (warps > 4) warps = 4;
+        }
+        if (warps >= 2) {
             static std::atomic<uint64_t> known[3];
             auto kern = rp == 4   ? norm_forward_kernel<T, W, ACC, VEC, 4>
                         : rp == 2 ? norm_forward_kernel<T, W, ACC, VEC, 2>
                                   : norm_forward_kernel<T, W, ACC, VEC, 1>;
-            const int warps = fit >= 12 ? 4 : fit < kFwdMostWarps ? (int)fit : kFwdMostWarps;
-            const int smem = (int)(kRingHeader + ring * warps);
-            const int64_t tiles = (a.rows + rp - 1) / rp, want = (tiles + warps - 1) / warps;
+            a.stages = (int)stages;
+            a.shared_params = share ? (int)params : 0;
+            const int smem = (int)(kRingHeader + a.shared_params + stages * tile * warps);
+            const int64_t want = (tiles + warps - 1) / warps;
             int64_t blocks = 0;
-            GT_CHECK(resident_blocks((const void *)kern, warps * 32, smem, kRingHeader + kFwdMostBytes, device,
+            GT_CHECK(resident_blocks((const void *)kern, (int)warps * 32, smem, kRingHeader + kFwdMostBytes, device,
                                      known[rp / 2], &blocks));
-            kern<<<(unsigned)(want < blocks ? want : blocks), warps * 32, smem, st>>>(a);
+            kern<<<(unsigned)(want < blocks ? want : blocks), (int)warps * 32, smem, st>>>(a);
             GT_CUDA(cudaGetLastError());
             note_launches(1);
             return 0;

@@ -4,8 +4,9 @@ expert, each with its gradients (the last section of include/gtmoe.h).
 
 Arguments are CUDA tensors of one device, contiguous, float64, float32 or
 bfloat16; a call runs on that device's current torch stream, waits for
-nothing and may be captured into a CUDA graph.  Misuse raises ``ValueError``,
-what the library refuses ``GtmoeError``."""
+nothing and may be captured into a CUDA graph.  Results carry no autograd
+graph: the gradients are the functions named so.  Misuse raises
+``ValueError``, what the library refuses ``GtmoeError``."""
 from __future__ import annotations
 
 import ctypes
@@ -105,7 +106,9 @@ def layer_norm(x, weight=None, bias=None, epsilon: float = 1e-6, out=None):
     code, wcode = _code(dtype), _code(wdt)
     if out is None:
         out = torch.empty_like(x)
-    po = _tensor("out", out, shape, dtype, dev)
+        po = out.data_ptr()
+    else:
+        po = _tensor("out", out, shape, dtype, dev)
     mean = torch.empty(rows, dtype=_stats_dtype(x), device=x.device)
     rstd = torch.empty_like(mean)
     check(_L.gtmoe_layer_norm(px, code, rows, width, pw, pb, wcode, epsilon, po, mean.data_ptr(), rstd.data_ptr(),
@@ -138,7 +141,9 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
         pres = _tensor("residual_gradients", residual_gradients, shape, dtype, dev)
     if input_gradients is None:
         input_gradients = torch.empty_like(g)
-    pdx = _tensor("input_gradients", input_gradients, shape, dtype, dev)
+        pdx = input_gradients.data_ptr()
+    else:
+        pdx = _tensor("input_gradients", input_gradients, shape, dtype, dev)
     if (weight_grad is None) != (bias_grad is None):
         raise ValueError("weight_grad and bias_grad are given together")
     accumulate = weight_grad is not None
@@ -148,8 +153,10 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
         if not accumulate:
             weight_grad = torch.empty(width, dtype=wdt, device=g.device)
             bias_grad = torch.empty_like(weight_grad)
-        pdw = _tensor("weight_grad", weight_grad, (width,), wdt, dev)
-        pdb = _tensor("bias_grad", bias_grad, (width,), wdt, dev)
+            pdw, pdb = weight_grad.data_ptr(), bias_grad.data_ptr()
+        else:
+            pdw = _tensor("weight_grad", weight_grad, (width,), wdt, dev)
+            pdb = _tensor("bias_grad", bias_grad, (width,), wdt, dev)
         need = ctypes.c_int64(0)
         check(_L.gtmoe_layer_norm_workspace(code, rows, width, ctypes.byref(need)))
         nbytes = need.value
@@ -171,7 +178,9 @@ def dropout(x, rate: float, seed: int, stream: int = 0, offset: int = 0, residua
     code = _code(dtype)
     if out is None:
         out = torch.empty_like(x)
-    po = _tensor("out", out, shape, dtype, dev)
+        po = out.data_ptr()
+    else:
+        po = _tensor("out", out, shape, dtype, dev)
     check(_L.gtmoe_dropout(px, pr, code, x.numel(), rate, seed, stream, offset, po, _stream(dev)))
     return out
 
@@ -186,7 +195,9 @@ def dropout_backward(output_gradients, rate: float, seed: int, stream: int = 0, 
     code = _code(g.dtype)
     if input_gradients is None:
         input_gradients = torch.empty_like(g)
-    pdx = _tensor("input_gradients", input_gradients, g.shape, g.dtype, dev)
+        pdx = input_gradients.data_ptr()
+    else:
+        pdx = _tensor("input_gradients", input_gradients, g.shape, g.dtype, dev)
     check(_L.gtmoe_dropout_backward(pg, code, g.numel(), rate, seed, stream, offset, pdx, _stream(dev)))
     return input_gradients
 
@@ -212,7 +223,9 @@ def grouped_product(x, weights, counts, out=None):
     code = _code(dtype)
     if out is None:
         out = torch.empty((rows, outputs), dtype=dtype, device=x.device)
-    po = _tensor("out", out, (rows, outputs), dtype, dev)
+        po = out.data_ptr()
+    else:
+        po = _tensor("out", out, (rows, outputs), dtype, dev)
     check(_L.gtmoe_grouped_product(px, pw, code, rows, inputs, outputs, groups, pc, po, _stream(dev)))
     return out
 
@@ -227,7 +240,9 @@ def grouped_product_input_gradients(output_gradients, weights, counts, input_gra
     code = _code(dtype)
     if input_gradients is None:
         input_gradients = torch.empty((rows, inputs), dtype=dtype, device=g.device)
-    pdx = _tensor("input_gradients", input_gradients, (rows, inputs), dtype, dev)
+        pdx = input_gradients.data_ptr()
+    else:
+        pdx = _tensor("input_gradients", input_gradients, (rows, inputs), dtype, dev)
     check(_L.gtmoe_grouped_product_input_grad(pg, pw, code, rows, inputs, outputs, groups, pc, pdx, _stream(dev)))
     return input_gradients
 
