@@ -9,16 +9,15 @@ namespace {
 
 __device__ int g_error;  // first code a kernel recorded since the last check
 
-constexpr int kStep = 16;   // terms of the sums per shared-memory step
 constexpr int kThreads = 256;
 
-// One operand of a tile: `n` values along the tile's axis by kStep terms.
+// One operand of a tile: TILE values along the tile's axis by STEP terms.
 // KMAJOR: the terms are contiguous in memory, else the tile's axis is.
 // Consecutive threads load along the contiguous axis, into registers while the
 // step before is multiplied, then into shared memory as [term][value].
-template <typename T, typename ACC, int TILE, bool KMAJOR>
+template <typename T, typename ACC, int TILE, int STEP, bool KMAJOR>
 struct Operand {
-    static constexpr int kLoads = TILE * kStep / kThreads;
+    static constexpr int kLoads = TILE * STEP / kThreads;
     const T *p;      // this thread's first value of step 0
     int64_t q_step, k_step;
     int at, term;    // its place in the tile
@@ -28,18 +27,18 @@ struct Operand {
     // base: value 0, term 0; ld: distance of the outer axis
     __device__ __forceinline__ void begin(const T *base, int64_t ld, int64_t n_values, int64_t n_terms) {
         const int t = threadIdx.x;
-        term = KMAJOR ? t % kStep : t / TILE;
-        at = KMAJOR ? t / kStep : t % TILE;
+        term = KMAJOR ? t % STEP : t / TILE;
+        at = KMAJOR ? t / STEP : t % TILE;
         p = base + (KMAJOR ? at * ld + term : term * ld + at);
-        q_step = (KMAJOR ? kThreads / kStep : kThreads / TILE) * ld;
-        k_step = KMAJOR ? kStep : kStep * ld;
+        q_step = (KMAJOR ? kThreads / STEP : kThreads / TILE) * ld;
+        k_step = KMAJOR ? STEP : STEP * ld;
         n = n_values;
         terms = n_terms;
     }
     __device__ __forceinline__ void load(int64_t k0) {
 #pragma unroll
         for (int q = 0; q < kLoads; q++) {
-            const int i = KMAJOR ? at + q * (kThreads / kStep) : at;
+            const int i = KMAJOR ? at + q * (kThreads / STEP) : at;
             const int64_t k = k0 + (KMAJOR ? term : term + q * (kThreads / TILE));
             v[q] = i < n && k < terms ? (ACC)p[q * q_step] : ACC(0);
         }
@@ -48,7 +47,7 @@ struct Operand {
     __device__ __forceinline__ void store(ACC (*s)[TILE + 4]) const {
 #pragma unroll
         for (int q = 0; q < kLoads; q++) {
-            if (KMAJOR) s[term][at + q * (kThreads / kStep)] = v[q];
+            if (KMAJOR) s[term][at + q * (kThreads / STEP)] = v[q];
             else s[term + q * (kThreads / TILE)][at] = v[q];
         }
     }
@@ -58,18 +57,20 @@ struct Operand {
 //   kProduct     i row, j output, p input:   A = X[i][p],  B = W_g[j][p]
 //   kInputGrad   i row, j input,  p output:  A = dY[i][p], B = W_g[p][j]
 //   kWeightGrad  i output, j input, p row:   A = dY[p][i], B = X[p][j]
-// TILE x TILE outputs per block, (TILE / 16)^2 per thread, each one sum in
-// ascending p in ACC.  Two buffers: one barrier per step.
-template <typename T, typename ACC, typename OUT, GroupedOp OP, int TILE>
+// TI x TJ outputs per block, (TI / 16) x (TJ / 16) per thread, each one sum in
+// ascending p in ACC, STEP terms per shared-memory step.  Two buffers: one
+// barrier per step.
+template <typename T, typename ACC, typename OUT, GroupedOp OP, int TI, int TJ, int STEP>
 __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const GroupedProduct a) {
-    constexpr int R = TILE / 16, V = R < 4 ? R : 4;  // outputs per thread and axis, in runs of V
-    __shared__ __align__(16) ACC sa[2][kStep][TILE + 4], sb[2][kStep][TILE + 4];
+    // outputs per thread and axis, in runs of VI and VJ
+    constexpr int RI = TI / 16, VI = RI < 4 ? RI : 4, RJ = TJ / 16, VJ = RJ < 4 ? RJ : 4;
+    __shared__ __align__(16) ACC sa[2][STEP][TI + 4], sb[2][STEP][TJ + 4];
     __shared__ int start[kMaxGroups + 1], tiles[kMaxGroups + 1], scratch[kThreads / 32];
     const int64_t n_j = OP == kProduct ? a.outputs : a.inputs;
-    const int64_t j_tiles = (n_j + TILE - 1) / TILE;
+    const int64_t j_tiles = (n_j + TJ - 1) / TJ;
     const bool ok = OP == kWeightGrad ? group_ranges(a.counts, a.groups, a.rows, kAnyRows, 1,
-                                                     (int)((a.outputs + TILE - 1) / TILE), start, tiles, scratch)
-                                      : group_ranges(a.counts, a.groups, a.rows, TILE, 0, 1, start, tiles, scratch);
+                                                     (int)((a.outputs + TI - 1) / TI), start, tiles, scratch)
+                                      : group_ranges(a.counts, a.groups, a.rows, TI, 0, 1, start, tiles, scratch);
     if (!ok && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_error, 0, kErrBadCounts);
     const int64_t total = (int64_t)tiles[a.groups] * j_tiles;
     const T *A = (const T *)a.a, *B = (const T *)a.b;
@@ -78,54 +79,51 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
     for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
         const int it = (int)(u / j_tiles);
         while (tiles[g + 1] <= it) g++;
-        const int64_t i0 = (int64_t)(it - tiles[g]) * TILE, j0 = (u % j_tiles) * TILE;
+        const int64_t i0 = (int64_t)(it - tiles[g]) * TI, j0 = (u % j_tiles) * TJ;
         const int64_t r0 = start[g], m = start[g + 1] - start[g];
         const int64_t i_end = OP == kWeightGrad ? a.outputs : m;
         const int64_t p_end = OP == kProduct ? a.inputs : OP == kInputGrad ? a.outputs : m;
         const T *Wg = B + (int64_t)g * a.outputs * a.inputs;
-        Operand<T, ACC, TILE, OP != kWeightGrad> oa;
-        Operand<T, ACC, TILE, OP == kProduct> ob;
+        Operand<T, ACC, TI, STEP, OP != kWeightGrad> oa;
+        Operand<T, ACC, TJ, STEP, OP == kProduct> ob;
         if (OP == kWeightGrad) oa.begin(A + r0 * a.outputs + i0, a.outputs, i_end - i0, p_end);
         else oa.begin(A + (r0 + i0) * p_end, p_end, i_end - i0, p_end);
         if (OP == kProduct) ob.begin(Wg + j0 * a.inputs, a.inputs, n_j - j0, p_end);
         else if (OP == kInputGrad) ob.begin(Wg + j0, a.inputs, n_j - j0, p_end);
         else ob.begin(B + r0 * a.inputs + j0, a.inputs, n_j - j0, p_end);
-        ACC acc[R][R] = {};
+        ACC acc[RI][RJ] = {};
         oa.load(0);
         ob.load(0);
         int buf = 0;
-        for (int64_t p0 = 0; p0 < p_end; p0 += kStep, buf ^= 1) {
+        for (int64_t p0 = 0; p0 < p_end; p0 += STEP, buf ^= 1) {
             oa.store(sa[buf]);
             ob.store(sb[buf]);
             __syncthreads();  // also: the step before last has been multiplied by every thread
-            if (p0 + kStep < p_end) {
-                oa.load(p0 + kStep);
-                ob.load(p0 + kStep);
+            if (p0 + STEP < p_end) {
+                oa.load(p0 + STEP);
+                ob.load(p0 + STEP);
             }
 #pragma unroll
-            for (int p = 0; p < kStep; p++) {
-                ACC ra[R], rb[R];
+            for (int p = 0; p < STEP; p++) {
+                ACC ra[RI], rb[RJ];
 #pragma unroll
-                for (int h = 0; h < R / V; h++)
+                for (int x = 0; x < RI; x++) ra[x] = sa[buf][p][x / VI * 16 * VI + ty * VI + x % VI];
 #pragma unroll
-                    for (int q = 0; q < V; q++) {
-                        ra[h * V + q] = sa[buf][p][h * 16 * V + ty * V + q];
-                        rb[h * V + q] = sb[buf][p][h * 16 * V + tx * V + q];
-                    }
+                for (int y = 0; y < RJ; y++) rb[y] = sb[buf][p][y / VJ * 16 * VJ + tx * VJ + y % VJ];
 #pragma unroll
-                for (int x = 0; x < R; x++)
+                for (int x = 0; x < RI; x++)
 #pragma unroll
-                    for (int y = 0; y < R; y++) acc[x][y] += ra[x] * rb[y];
+                    for (int y = 0; y < RJ; y++) acc[x][y] += ra[x] * rb[y];
             }
         }
         __syncthreads();  // the buffers are free for the next tile
         OUT *C = (OUT *)a.c;
         const int64_t base = OP == kWeightGrad ? (int64_t)g * a.outputs * a.inputs : r0 * n_j;
 #pragma unroll
-        for (int x = 0; x < R; x++)
+        for (int x = 0; x < RI; x++)
 #pragma unroll
-            for (int y = 0; y < R; y++) {
-                const int64_t i = i0 + x / V * 16 * V + ty * V + x % V, j = j0 + y / V * 16 * V + tx * V + y % V;
+            for (int y = 0; y < RJ; y++) {
+                const int64_t i = i0 + x / VI * 16 * VI + ty * VI + x % VI, j = j0 + y / VJ * 16 * VJ + tx * VJ + y % VJ;
                 if (i < i_end && j < n_j) {
                     OUT &o = C[base + i * n_j + j];
                     o = (OUT)(OP == kWeightGrad && a.accumulate ? (ACC)o + acc[x][y] : acc[x][y]);
@@ -134,34 +132,40 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
     }
 }
 
-template <typename T, typename ACC, typename OUT, GroupedOp OP, int TILE>
-int launch_simt_tile(const GroupedProduct &p, int64_t *tiles, cudaStream_t st) {
+// At most this many tiles: the rows of a group end inside a tile.
+template <GroupedOp OP>
+int64_t most_tiles(const GroupedProduct &p, int ti, int tj) {
     const int64_t n_j = OP == kProduct ? p.outputs : p.inputs;
-    // at most this many tiles: the rows of a group end inside a tile
-    const int64_t i_tiles = OP == kWeightGrad ? (int64_t)p.groups * ((p.outputs + TILE - 1) / TILE)
-                                              : p.rows / TILE + (p.rows < p.groups ? p.rows : p.groups);
-    const int64_t most = i_tiles * ((n_j + TILE - 1) / TILE);
-    if (tiles) {
-        *tiles = most;
-        return 0;
-    }
+    const int64_t i_tiles = OP == kWeightGrad ? (int64_t)p.groups * ((p.outputs + ti - 1) / ti)
+                                              : p.rows / ti + (p.rows < p.groups ? p.rows : p.groups);
+    return i_tiles * ((n_j + tj - 1) / tj);
+}
+
+template <typename T, typename ACC, typename OUT, GroupedOp OP, int TI, int TJ, int STEP>
+int launch_simt_tile(const GroupedProduct &p, cudaStream_t st) {
+    const int64_t most = most_tiles<OP>(p, TI, TJ);
     const unsigned grid = (unsigned)(most < 148 * 16 ? most : 148 * 16);
-    grouped_simt_product_kernel<T, ACC, OUT, OP, TILE><<<grid, kThreads, 0, st>>>(p);
+    grouped_simt_product_kernel<T, ACC, OUT, OP, TI, TJ, STEP><<<grid, kThreads, 0, st>>>(p);
     GT_CUDA(cudaGetLastError());
     note_launches(1);
     return 0;
 }
 
-// Tiles of 128 x 128 (64 products per 16 values read) once they are enough for
-// every SM, else of 64 x 64; float64 has shared memory for the latter only.
+// Groups of few rows on average: tiles of 32 rows, and twice the terms per
+// step, since the steps' latencies are what a block then waits for.  Else tiles
+// of 128 x 128 (64 products per 16 values read) once they are enough for every
+// SM and the groups fill them, else of 64 x 64; float64 has shared memory for
+// the latter only.
 template <typename T, typename ACC, typename OUT, GroupedOp OP>
 int launch_simt(const GroupedProduct &p, cudaStream_t st) {
     if constexpr (sizeof(ACC) == 4) {
-        int64_t tiles = 0;
-        GT_CHECK((launch_simt_tile<T, ACC, OUT, OP, 128>(p, &tiles, st)));
-        if (tiles >= 2 * 148) return launch_simt_tile<T, ACC, OUT, OP, 128>(p, nullptr, st);
+        const int64_t average = p.rows / p.groups;
+        if constexpr (OP != kWeightGrad)
+            if (average < 48) return launch_simt_tile<T, ACC, OUT, OP, 32, 64, 32>(p, st);
+        if ((OP == kWeightGrad || average >= 96) && most_tiles<OP>(p, 128, 128) >= 2 * 148)
+            return launch_simt_tile<T, ACC, OUT, OP, 128, 128, 16>(p, st);
     }
-    return launch_simt_tile<T, ACC, OUT, OP, 64>(p, nullptr, st);
+    return launch_simt_tile<T, ACC, OUT, OP, 64, 64, 16>(p, st);
 }
 
 template <typename T, typename ACC>
