@@ -41,6 +41,11 @@
 // (leader), warps 2-9 epilogue (TMEM -> bf16 / float32 -> shared memory ->
 // coalesced rows), warp 10 loads B, warp 11 zeroes row tails.  Two accumulators: the epilogue of a tile
 // overlaps the next tile's products.  Every wait is bounded as in tc.cu.
+//
+// Measured (B200, in loops of most of a second, at the power cap): 8192^3 1302
+// TF/s (cuBLAS 1373); 64 groups of 1536 rows, 2048 x 2048, product and input
+// gradient 1217 TF/s (cuBLAS's batched product 1234), float32 weight gradient
+// 1081; 384 rows in 64 groups, 2048 -> 1408, 71.5 us = 5.2 TB/s of weights.
 #include <atomic>
 
 #include "grouped.h"
@@ -667,7 +672,7 @@ View chunks(int64_t rows, int64_t cols) {
 // Rows of a group per unit of the weight gradient.  With tiles for every CTA
 // pair a unit has all of a group's rows; with fewer the groups are split, into
 // about two units per pair, and the parts' sums added by a second kernel
-// (1 group of 65536 rows, 512 x 512: 467 us unsplit).  Short groups are not:
+// (1 group of 65536 rows, 512 x 512: 467 -> 53 us).  Short groups are not:
 // their units end before the second kernel would.
 int part_rows(int64_t rows, int64_t inputs, int64_t outputs, int groups) {
     const int64_t area = ((outputs + kTileM - 1) / kTileM) * ((inputs + kTileN - 1) / kTileN);

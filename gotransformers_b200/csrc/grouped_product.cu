@@ -59,7 +59,8 @@ struct Operand {
 //   kWeightGrad  i output, j input, p row:   A = dY[p][i], B = X[p][j]
 // TI x TJ outputs per block, (TI / 16) x (TJ / 16) per thread, each one sum in
 // ascending p in ACC, STEP terms per shared-memory step.  Two buffers: one
-// barrier per step.
+// barrier per step.  FFMA-bound: 16384 rows in 8 groups, 1024 x 1024, float32
+// 45 TF/s (cuBLAS's float32 product of this size of sums 57).
 template <typename T, typename ACC, typename OUT, GroupedOp OP, int TI, int TJ, int STEP>
 __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const GroupedProduct a) {
     // outputs per thread and axis, in runs of VI and VJ
