@@ -75,8 +75,9 @@ constexpr int kChunkRows = 16;
 constexpr int kRowPitch = 272;
 constexpr int kRowBuf = kChunkRows * kRowPitch;
 constexpr int kGradPitch = 36;
-constexpr int kEpiBytes = kEpiWarps * 32 * kGradPitch * 4;
-static_assert(4 * kRowBuf <= kEpiBytes, "epilogue staging");
+constexpr int kWarpBuf = 5 * 1024;  // swizzled tiles start on 1024 bytes
+constexpr int kEpiBytes = kEpiWarps * kWarpBuf;
+static_assert(4 * kRowBuf <= kEpiBytes && 32 * kGradPitch * 4 <= kWarpBuf, "epilogue staging");
 constexpr int kBarBytes = 256;
 constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiBytes + kBarBytes + (2 * (kMaxGroups + 1) + kThreads / 32) * 4;
 static_assert(kSmemBytes <= 232448, "shared memory per CTA");
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!add) {
                     // TMA writes the rows out, and leaves out what lies past the last row and column: the LSU path
                     // below costs the shared memory that feeds the MMAs twice the traffic
-                    const uint32_t buf_addr = smem_u32(epi) + (warp - 2) * 4096;
+                    const uint32_t buf_addr = smem_u32(epi) + (warp - 2) * kWarpBuf;
                     const int m0 = m_first + quad * 32, n0 = w.n0 + group * kHalf;
                     const int per = f32 ? 32 : 64;  // columns in 128 bytes
 #pragma unroll
@@ -544,7 +545,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     continue;
                 }
-                float *stage = reinterpret_cast<float *>(epi) + (warp - 2) * 32 * kGradPitch;
+                float *stage = reinterpret_cast<float *>(epi + (warp - 2) * kWarpBuf);
+                // a unit before, of a group that was split, may have left a store that still reads the buffer
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
                 void *base = w.part >= 0 ? (void *)a.parts : a.out;
                 const int64_t o0 = ((int64_t)(w.part >= 0 ? w.part : w.g) * a.outputs + m_first + quad * 32) * a.inputs +
                                    w.n0 + group * kHalf;

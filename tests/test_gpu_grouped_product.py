@@ -115,6 +115,23 @@ def test_weight_gradients_whose_sums_are_split(counts, inputs, outputs):
         assert torch.equal(dw.cpu(), (ref + before.double()).to(dtype))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_split_and_whole_groups_added_to(dtype):
+    """One CTA pair's units go back and forth between parts of a split group,
+    which TMA stores, and groups that are added to from shared memory: the two
+    share the epilogue's buffers."""
+    counts = [9000, 5, 300, 7001, 64, 1, 8192, 700, 4097, 2]
+    x, _, dy = make(counts, 520, 264, BF16, 21, whole=True)
+    X, DY, C = x.cuda(), dy.cuda(), device_counts(counts)
+    ref = R.grouped_weight_gradients(dy, x, counts)
+    before = torch.randint(-9, 10, ref.shape).to(dtype)
+    want = (ref + before.double()).to(dtype)
+    for _ in range(20):
+        dw = before.cuda()
+        moe.grouped_product_weight_gradients(DY, X, C, weight_grad=dw)
+        assert torch.equal(dw.cpu(), want)
+
+
 @pytest.mark.parametrize("rows,groups", [(1536, 1), (65536, 1), (20000, 3), (40000, 80)])
 def test_float32_weight_gradients_keep_their_digits(rows, groups):
     """Runs of 768 rows are 48 additions that cut at most 2^-23 of the sum
