@@ -545,13 +545,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     continue;
                 }
+                // added to what is there: coalesced reads and writes by way of shared memory
                 float *stage = reinterpret_cast<float *>(epi + (warp - 2) * kWarpBuf);
                 // a unit before, of a group that was split, may have left a store that still reads the buffer
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
-                void *base = w.part >= 0 ? (void *)a.parts : a.out;
-                const int64_t o0 = ((int64_t)(w.part >= 0 ? w.part : w.g) * a.outputs + m_first + quad * 32) * a.inputs +
-                                   w.n0 + group * kHalf;
+                const int64_t o0 = ((int64_t)w.g * a.outputs + m_first + quad * 32) * a.inputs + w.n0 + group * kHalf;
                 const int rows = a.outputs - m_first - quad * 32;  // of dW for this warp
 #pragma unroll
                 for (int c = 0; c < kHalf / 32; c++) {
@@ -565,38 +564,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (f32) {
                         const int cc = (lane & 7) * 4;
-                        float *out = (float *)base + o0 + c * 32 + cc;
+                        float *out = (float *)a.out + o0 + c * 32 + cc;
 #pragma unroll
                         for (int q = 0; q < 8; q++) {
                             const int r = q * 4 + (lane >> 3);
                             if (r < rows && c * 32 + cc < left) {
                                 float4 *p = reinterpret_cast<float4 *>(out + (int64_t)r * a.inputs);
-                                float4 x = *reinterpret_cast<const float4 *>(stage + r * kGradPitch + cc);
-                                if (add) {
-                                    const float4 b = *p;
-                                    x.x += b.x, x.y += b.y, x.z += b.z, x.w += b.w;
-                                }
-                                *p = x;
+                                const float4 x = *reinterpret_cast<const float4 *>(stage + r * kGradPitch + cc), b = *p;
+                                *p = make_float4(x.x + b.x, x.y + b.y, x.z + b.z, x.w + b.w);
                             }
                         }
                     } else {
                         using Io = VecIO<__nv_bfloat16, float, 8>;
                         const int cc = (lane & 3) * 8;
-                        __nv_bfloat16 *out = (__nv_bfloat16 *)base + o0 + c * 32 + cc;
+                        __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + o0 + c * 32 + cc;
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
                             const int r = q * 8 + (lane >> 2);
                             if (r < rows && c * 32 + cc < left) {
                                 __nv_bfloat16 *p = out + (int64_t)r * a.inputs;
-                                float x[8], b[8];
+                                float b[8];
+                                Io::unpack(Io::load(p), b);
 #pragma unroll
-                                for (int i = 0; i < 8; i++) x[i] = stage[r * kGradPitch + cc + i];
-                                if (add) {
-                                    Io::unpack(Io::load(p), b);
-#pragma unroll
-                                    for (int i = 0; i < 8; i++) x[i] += b[i];
-                                }
-                                Io::store(p, x);
+                                for (int i = 0; i < 8; i++) b[i] += stage[r * kGradPitch + cc + i];
+                                Io::store(p, b);
                             }
                         }
                     }
