@@ -120,7 +120,8 @@ GTMOE_API int gtmoe_create_ep(const gtmoe_config *cfg, int device, int n_ranks, 
 GTMOE_API int gtmoe_ep_set_replicas(gtmoe_t h, int n, const int32_t *experts);
 
 /* The mixture-of-experts half of transformer.Block.Forward (block.go:72-77,
- * no hyper-connections, dropout off): out = x + Forward(RMSNorm(x)), in one
+ * no hyper-connections, dropout off unless gtmoe_set_dropout gave a rate):
+ * out = x + Forward(RMSNorm(x)), in one
  * call.  gtmoe_set_norm sets the block's FeedForwardNorm (RMSNorm weights,
  * d_model float64, and epsilon; normalization/rmsnorm.go:10-31);
  * gtmoe_forward_block normalizes on the GPU in float64 exactly as
@@ -353,7 +354,8 @@ GTMOE_API int gtmoe_dropout_backward(const void *dout, int dtype, int64_t n, dou
 /* Dropout inside gtmoe_forward_block: out = x + dropout(Forward(RMSNorm(x)))
  * from now on, with the decisions of gtmoe_dropout over the T x d values at
  * offset 0.  A training step gives every step its own stream_id; rate 0 (the
- * start) switches it off.  The gradient of the mixture's output, which
+ * start) switches it off.  The mixture's output is rounded to x's dtype, as
+ * gtmoe_forward returns it, before it is dropped.  Its gradient, which
  * gtmoe_backward takes, is then gtmoe_dropout_backward's. */
 GTMOE_API int gtmoe_set_dropout(gtmoe_t h, double rate, uint64_t seed, uint64_t stream_id);
 
