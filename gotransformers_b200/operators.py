@@ -86,6 +86,11 @@ def _stream(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def _dtype(a):
+    """a's dtype; None for what is no tensor, which the checks then refuse."""
+    return getattr(a, "dtype", None)
+
+
 def _stats_dtype(x):
     return torch.float64 if x.dtype is torch.float64 else torch.float32
 
@@ -98,9 +103,9 @@ def layer_norm(x, weight=None, bias=None, epsilon: float = 1e-6, out=None):
     px, dev = _rows("x", x)
     shape, dtype = x.shape, x.dtype
     rows, width = shape
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"weight and bias must have one dtype, got {weight.dtype} and {bias.dtype}")
-    wdt = weight.dtype if weight is not None else bias.dtype if bias is not None else dtype
+    wdt = _dtype(weight) if weight is not None else _dtype(bias) if bias is not None else dtype
+    if weight is not None and bias is not None and wdt != _dtype(bias):
+        raise ValueError(f"weight and bias must be tensors of one dtype, got {wdt} and {_dtype(bias)}")
     pw = None if weight is None else _tensor("weight", weight, (width,), wdt, dev)
     pb = None if bias is None else _tensor("bias", bias, (width,), wdt, dev)
     code, wcode = _code(dtype), _code(wdt)
@@ -133,8 +138,7 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
     px = _tensor("x", x, shape, dtype, dev)
     sdt = _stats_dtype(g)
     pm, pr = _tensor("mean", mean, (rows,), sdt, dev), _tensor("rstd", rstd, (rows,), sdt, dev)
-    wdt = weight.dtype if weight is not None else weight_grad.dtype if weight_grad is not None else sdt
-    wcode = _code(wdt)
+    wdt = _dtype(weight) if weight is not None else _dtype(weight_grad) if weight_grad is not None else sdt
     pw = None if weight is None else _tensor("weight", weight, (width,), wdt, dev)
     pres = None
     if residual_gradients is not None:
@@ -147,6 +151,7 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
     if (weight_grad is None) != (bias_grad is None):
         raise ValueError("weight_grad and bias_grad are given together")
     accumulate = weight_grad is not None
+    wcode = _code(wdt)
     pdw = pdb = pwork = None
     nbytes = 0
     if accumulate or want_parameters:
@@ -265,10 +270,11 @@ def grouped_product_weight_gradients(output_gradients, x, counts, weight_grad=No
     accumulate = weight_grad is not None
     if not accumulate:
         weight_grad = torch.empty((groups, outputs, inputs), dtype=dtype or g.dtype, device=g.device)
-    elif dtype is not None and weight_grad.dtype != dtype:
-        raise ValueError(f"weight_grad is {weight_grad.dtype} but dtype {dtype}")
-    wcode = _code(weight_grad.dtype)
-    pdw = _tensor("weight_grad", weight_grad, (groups, outputs, inputs), weight_grad.dtype, dev)
+    wdt = _dtype(weight_grad)
+    if dtype is not None and wdt != dtype:
+        raise ValueError(f"weight_grad is {wdt} but dtype {dtype}")
+    pdw = _tensor("weight_grad", weight_grad, (groups, outputs, inputs), wdt, dev)
+    wcode = _code(wdt)
     need, pwork = ctypes.c_int64(0), None
     check(_L.gtmoe_grouped_product_workspace(code, rows, inputs, outputs, groups, ctypes.byref(need)))
     if need.value:

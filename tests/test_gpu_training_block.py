@@ -180,3 +180,31 @@ def test_block_step_with_dropout(prec, T, dtype, on_device):
     with pytest.raises(_lib.GtmoeError):
         m.set_dropout(1.0)
     m.close()
+
+
+@pytest.mark.parametrize("other", [1.0, [1.0] * 64, np.ones(64, np.float32)], ids=["number", "list", "array"])
+def test_parameters_that_are_no_tensors_are_refused(other):
+    """ValueError, as for every other misuse, wherever a tensor is expected."""
+    x = torch.ones(8, 64, device="cuda")
+    counts = torch.tensor([8], device="cuda")
+    w = torch.ones(64, device="cuda")
+    y, mean, rstd = moe.layer_norm(x, w, w)
+    calls = [
+        lambda: moe.layer_norm(other),
+        lambda: moe.layer_norm(x, other, w),
+        lambda: moe.layer_norm(x, w, other),
+        lambda: moe.layer_norm(x, None, other),
+        lambda: moe.layer_norm(x, w, w, out=other),
+        lambda: moe.layer_norm_backward(y, x, mean, rstd, other),
+        lambda: moe.layer_norm_backward(y, x, other, rstd, w),
+        lambda: moe.layer_norm_backward(y, x, mean, rstd, None, None, None, other, other),
+        lambda: moe.layer_norm_backward(y, x, mean, rstd, w, residual_gradients=other),
+        lambda: moe.dropout(x, 0.5, 1, residual=other),
+        lambda: moe.grouped_product(x, other, counts),
+        lambda: moe.grouped_product(x, torch.ones(1, 64, 64, device="cuda"), other),
+        lambda: moe.grouped_product_weight_gradients(y, x, other),
+        lambda: moe.grouped_product_weight_gradients(y, x, counts, other),
+    ]
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()
