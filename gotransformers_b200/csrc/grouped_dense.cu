@@ -34,8 +34,12 @@
 // 6.6e-5 at 65536 rows), far more than float32 rounding.  The weight gradient,
 // whose result may be float32 and whose sums are the long ones, is therefore
 // accumulated in runs of kRunStages stages; the epilogue adds the runs in
-// registers, with rounding, while the next run is multiplied.  Results in bf16
-// keep one sum: their rounding is 2^-9.
+// registers, with rounding, while the next run is multiplied.  Results in bf16,
+// whose rounding is 2^-8, keep one sum up to kOneSumStages stages; beyond, the
+// loss grows faster than the rows (positive values, relative: 7.5e-5 at 65536
+// rows, 4.9e-4 at 262144, 7.0e-3 at 1048576) and runs take 2 to 6 % longer.
+// The sums over inputs and outputs have no runs: longer ones than
+// kMostSumTerms are not for this kernel.
 //
 // Persistent kernel, one CTA per SM; warp 0 loads A, warp 1 issues the MMAs
 // (leader), warps 2-9 epilogue (TMEM -> bf16 / float32 -> shared memory ->
@@ -63,6 +67,8 @@ constexpr int kTileM = 2 * kHalf, kTileN = 2 * kHalf;
 constexpr int kOperandBytes = kHalf * kStageK * 2;  // 16 KB
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kRunStages = 12;           // stages of the weight gradient's sums per run (768 rows)
+constexpr int kOneSumStages = 1024;      // 65536 rows
+constexpr int64_t kMostSumTerms = 1 << 18;
 constexpr int kChunkBytes = kStageK * 128;  // 64 columns x 64 terms of an M- or N-major operand
 constexpr int kEpiWarps = 8;             // two groups of four (one per TMEM lane quadrant), half the columns each
 constexpr int kThreads = (4 + kEpiWarps) * 32;
@@ -89,7 +95,7 @@ struct DenseArgs {
     int inputs, outputs;
     void *out;
     int out_f32, accumulate;
-    int sum_runs;   // kWeightGrad: float32 sums over runs of stages
+    int sum_runs;   // kWeightGrad: float32 sums over runs of stages (else for long groups only)
     int part_rows;  // kWeightGrad: rows of a group per unit
     float *parts;   // and where the sums of a group's parts go if it has several
 };
@@ -266,6 +272,12 @@ struct Units {
     }
 };
 
+// Stages of a unit's sum between two additions in registers.
+template <GroupedOp OP>
+__device__ __forceinline__ int run_stages_of(const DenseArgs &a, const Unit &w) {
+    return OP == kWeightGrad && (a.sum_runs || w.stages > kOneSumStages) ? kRunStages : w.stages;
+}
+
 // The tensor maps of a launch.  a, b: the whole boxes (two 64-column chunks of
 // an M- or N-major operand); a_edge, b_edge: one chunk; b_rows: rows of a
 // K-major B in boxes of 32 and 64 rows.
@@ -407,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int64_t u = cluster; u < total && ok; u += n_clusters) {
                 const Unit w = units.at(u);
                 const uint32_t idesc = instr_desc<OP>(w.n);
-                const int run_stages = OP == kWeightGrad && a.sum_runs ? kRunStages : w.stages;
+                const int run_stages = run_stages_of<OP>(a, w);
                 for (int s0 = 0; s0 < w.stages && ok; s0 += run_stages, run++) {
                     const uint32_t acc = run & 1, d = tmem_base + acc * kTileN;
                     ok = __all_sync(0xffffffffu, wait_for(&tmem_empty[acc], ((run >> 1) & 1) ^ 1, ab, 2));
@@ -486,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
                 // lanes are rows of dW; the runs' sums in registers
-                const int run_stages = a.sum_runs ? kRunStages : w.stages;
+                const int run_stages = run_stages_of<OP>(a, w);
                 float sum[kHalf];
 #pragma unroll
                 for (int i = 0; i < kHalf; i++) sum[i] = 0.f;
@@ -805,7 +817,8 @@ bool grouped_dense_usable(const GroupedProduct &p) {
     // TMA: rows and bases on 16 bytes; the epilogue stores 16 bytes.  A sum
     // over no rows at all has nothing to map.  A launch's tiles are counted in 31 bits.
     const int64_t m_tiles = (p.outputs + kTileM - 1) / kTileM, n_tiles = (p.inputs + kTileN - 1) / kTileN;
-    return p.dtype == GTMOE_DTYPE_BF16 && p.rows > 0 && p.inputs % 8 == 0 && p.outputs % 8 == 0 && aligned16(p.a) &&
+    const int64_t terms = p.op == kProduct ? p.inputs : p.op == kInputGrad ? p.outputs : 0;
+    return p.dtype == GTMOE_DTYPE_BF16 && p.rows > 0 && terms <= kMostSumTerms && p.inputs % 8 == 0 && p.outputs % 8 == 0 && aligned16(p.a) &&
            aligned16(p.b) && aligned16(p.c) && m_tiles * n_tiles < 0x7ffffffe / p.groups;
 }
 

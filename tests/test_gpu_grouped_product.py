@@ -144,6 +144,46 @@ def test_float32_weight_gradients_keep_their_digits(rows, groups):
     R.near("dw", dw, R.grouped_weight_gradients(dy, x, counts), 48 * 2.0**-23 + 86 * 2.0**-24)
 
 
+def positive(rows, columns, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (0.75 + 0.5 * torch.rand(rows, columns, generator=g, device="cuda")).to(BF16)
+
+
+def test_bfloat16_weight_gradients_of_long_groups():
+    """Values of one sign, whose sums lose the most where additions are cut: a
+    million rows in one sum would be 7.0e-3 short.  In runs of 768 rows it is
+    48 cut additions of at most 2^-23 and 1366 rounded ones, then the rounding
+    to bfloat16.  80 groups: the sums are not split."""
+    counts = [(1 << 20) + 37, 5] + [0] * 77 + [70000]
+    x, dy = positive(sum(counts), 64, 1), positive(sum(counts), 72, 2)
+    for dtype in (BF16, F32):
+        dw = moe.grouped_product_weight_gradients(dy, x, device_counts(counts), dtype=dtype)
+        at = 0
+        for g, n in enumerate(counts):
+            ref = dy[at:at + n].double().T @ x[at:at + n].double()
+            at += n
+            tol = R.HALF[dtype] + 48 * 2.0**-23 + 1367 * 2.0**-24
+            R.within(f"dw[{g}]", dw[g].cpu(), ref.cpu(), tol * ref.abs().cpu())
+    moe.check_operators()
+
+
+@pytest.mark.parametrize("direction", ["product", "input gradients"])
+def test_sums_over_very_long_rows(direction):
+    """A million products of one sign per value.  Rounded additions err
+    independently: beyond 8 * sqrt(n) * 2^-24 of the sum with a probability of
+    2 exp(-32) per value (one sum on the tensor cores would be 7e-3 short)."""
+    n, counts = 1 << 20, [3, 29]
+    x, w = positive(32, n, 3), positive(2 * 8, n, 4).view(2, 8, n)
+    if direction == "product":
+        y = moe.grouped_product(x, w, device_counts(counts))
+    else:
+        y = moe.grouped_product_input_gradients(x, w.transpose(1, 2).contiguous(), device_counts(counts))
+    for g, r in ((0, slice(0, 3)), (1, slice(3, 32))):
+        ref = x[r].double() @ w[g].double().T
+        R.within("y", y[r].cpu(), ref.cpu(), (R.HALF[BF16] + 8 * 2.0**10 * 2.0**-24) * ref.abs().cpu())
+    moe.check_operators()
+
+
 def test_many_groups():
     g = torch.Generator().manual_seed(8)
     counts = torch.randint(0, 6, (1024,), generator=g).tolist()
