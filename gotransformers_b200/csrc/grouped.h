@@ -101,6 +101,16 @@ __device__ __forceinline__ bool group_ranges(const int64_t *__restrict__ counts,
     return __syncthreads_and(ok);
 }
 
+// Adds `part`, the sum of a run of terms, to `total`; what the addition rounds
+// off is where the next run starts from (Knuth's two-sum), so that a sum's
+// error is that of its runs however many they are.
+__device__ __forceinline__ void fold(float &total, float &part) {
+    const float t = __fadd_rn(total, part), b = __fsub_rn(t, total);
+    const float off = __fadd_rn(__fsub_rn(total, __fsub_rn(t, b)), __fsub_rn(part, b));
+    total = t;
+    part = isfinite(t) ? off : 0.f;  // an infinite sum has no remainder
+}
+
 // The tensor-core kernel, and whether it takes these sizes, types and
 // addresses.
 bool grouped_dense_usable(const GroupedProduct &p);

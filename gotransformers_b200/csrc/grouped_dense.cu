@@ -29,17 +29,21 @@
 // each CTA zeroes the rows past the group's end of both operands before the MMA
 // (0 * NaN is NaN, so one operand would not do).
 //
-// The tensor cores cut every addition to an accumulator towards zero: over n
-// rows the sums shrink by about n / 16 * 2^-24.2 (measured: 4.0e-7 at 512 rows,
-// 6.6e-5 at 65536 rows), far more than float32 rounding.  The weight gradient,
-// whose result may be float32 and whose sums are the long ones, is therefore
-// accumulated in runs of kRunStages stages; the epilogue adds the runs in
-// registers, with rounding, while the next run is multiplied.  Results in bf16,
-// whose rounding is 2^-8, keep one sum up to kOneSumStages stages; beyond, the
-// loss grows faster than the rows (positive values, relative: 7.5e-5 at 65536
-// rows, 4.9e-4 at 262144, 7.0e-3 at 1048576) and runs take 2 to 6 % longer.
-// The sums over inputs and outputs have no runs: longer ones than
-// kMostSumTerms are not for this kernel.
+// The tensor cores cut every addition to an accumulator towards zero, so that a
+// sum made in one accumulator comes out short, by more the longer it is.
+// Measured: float32 results of normal values 4.0e-7 over 512 terms and 6.2e-7
+// over 768 (a float32 sum with rounding errs by 2e-7 to 4e-7, to both sides);
+// values of one sign 2.4e-5 over 8192 terms, 6.6e-5 over 65536, 1.6e-3 over
+// 262144, 7.0e-3 over 1048576 (bf16's half step is 3.9e-3).  Sums are therefore
+// made in runs of stages, which the epilogue adds in registers, with rounding,
+// while the next run is multiplied.  Float32 results in runs of 512 terms: of
+// 768 they took 1.5 % less time and erred by 6.8e-7 instead of 4.5e-7; of 256
+// they took 14 % more, as the epilogue needs about five stages to add a run up.
+// Results in bf16 in runs of 8192 terms, which cost less than 1 %; products
+// whose sums are no longer than that have a kernel without the registers for it.
+// Every 16 runs join a total in local memory, and what that addition rounds off
+// is carried on (fold(), grouped.h): equal rows would otherwise be rounded
+// alike every time (1.6e-4 over 16777216 rows).
 //
 // Persistent kernel, one CTA per SM; warp 0 loads A, warp 1 issues the MMAs
 // (leader), warps 2-9 epilogue (TMEM -> bf16 / float32 -> shared memory ->
@@ -66,9 +70,10 @@ constexpr int kHalf = 128;               // rows of A, and most rows of B, per C
 constexpr int kTileM = 2 * kHalf, kTileN = 2 * kHalf;
 constexpr int kOperandBytes = kHalf * kStageK * 2;  // 16 KB
 constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kRunStages = 12;           // stages of the weight gradient's sums per run (768 rows)
-constexpr int kOneSumStages = 1024;      // 65536 rows
-constexpr int64_t kMostSumTerms = 1 << 18;
+constexpr int kRunStages = 8;            // stages per run of a float32 weight gradient's sums (512 rows)
+constexpr int kLongRunStages = 128;      // and of sums rounded to bf16 (8192 terms)
+constexpr int kFoldRuns = 16;            // runs added up in a register before they join the total
+constexpr int kPartStep = 768;           // rows of a part of a group: a multiple of this
 constexpr int kChunkBytes = kStageK * 128;  // 64 columns x 64 terms of an M- or N-major operand
 constexpr int kEpiWarps = 8;             // two groups of four (one per TMEM lane quadrant), half the columns each
 constexpr int kThreads = (4 + kEpiWarps) * 32;
@@ -273,9 +278,9 @@ struct Units {
 };
 
 // Stages of a unit's sum between two additions in registers.
-template <GroupedOp OP>
+template <GroupedOp OP, bool RUNS>
 __device__ __forceinline__ int run_stages_of(const DenseArgs &a, const Unit &w) {
-    return OP == kWeightGrad && (a.sum_runs || w.stages > kOneSumStages) ? kRunStages : w.stages;
+    return !RUNS ? w.stages : OP == kWeightGrad && a.sum_runs ? kRunStages : kLongRunStages;
 }
 
 // The tensor maps of a launch.  a, b: the whole boxes (two 64-column chunks of
@@ -286,7 +291,8 @@ struct Maps {
     CUtensorMap a, b, a_edge, b_edge, b_rows[2], out, parts;
 };
 
-template <GroupedOp OP>
+// RUNS: sums may have several runs of stages (always so for kWeightGrad).
+template <GroupedOp OP, bool RUNS>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_dense_kernel(const __grid_constant__ Maps maps, const DenseArgs a) {
     extern __shared__ uint8_t smem_raw[];
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int64_t u = cluster; u < total && ok; u += n_clusters) {
                 const Unit w = units.at(u);
                 const uint32_t idesc = instr_desc<OP>(w.n);
-                const int run_stages = run_stages_of<OP>(a, w);
+                const int run_stages = run_stages_of<OP, RUNS>(a, w);
                 for (int s0 = 0; s0 < w.stages && ok; s0 += run_stages, run++) {
                     const uint32_t acc = run & 1, d = tmem_base + acc * kTileN;
                     ok = __all_sync(0xffffffffu, wait_for(&tmem_empty[acc], ((run >> 1) & 1) ^ 1, ab, 2));
@@ -460,11 +466,79 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(tmem_empty_leader + acc * (uint32_t)sizeof(uint64_t));
         };
+        // this warp's part of a unit's D, its runs added up with rounding; false when a wait gave up
+        auto add_runs = [&](const Unit &w, int left, float (&sum)[kHalf]) {
+            const int run_stages = run_stages_of<OP, RUNS>(a, w);
+            float folded[kHalf];  // in local memory, which units of at most kFoldRuns runs do not touch
+            int at = 0, runs = 0;
+            asm volatile("" : "+r"(at));
+#pragma unroll
+            for (int i = 0; i < kHalf; i++) sum[i] = 0.f;
+            for (int s0 = 0; s0 < w.stages; s0 += run_stages, run++, runs++) {
+                if (runs && runs % kFoldRuns == 0) {
+                    if (runs == kFoldRuns)
+#pragma unroll
+                        for (int i = 0; i < kHalf; i++) folded[at + i] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kHalf; i++) {
+                        fold(folded[at + i], sum[i]);
+                        if (i % 4 == 3) asm volatile("" ::: "memory");  // few loads at once: the registers are taken
+                    }
+                }
+                const uint32_t acc = run & 1;
+                const bool ready = wait_for(&tmem_full[acc], (run >> 1) & 1, ab, 4);
+                if (!epi_vote(group, ready)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < kHalf / 16; c++)
+                    if (c * 16 < left) {
+                        uint32_t v[16];
+                        tmem_ld16(t_warp + acc * kTileN + c * 16, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; i++) sum[c * 16 + i] += __uint_as_float(v[i]);
+                    }
+                release(acc);
+            }
+            if (runs > kFoldRuns)
+#pragma unroll
+                for (int i = 0; i < kHalf; i++) {
+                    sum[i] += folded[at + i];
+                    if (i % 4 == 3) asm volatile("" ::: "memory");
+                }
+            return true;
+        };
+        // 16 rows of bf16 outputs: a lane has one output feature, value(i) that of row i of the chunk
+        auto store_rows = [&](const Unit &w, int c, int m_first, int left, auto value) {
+            uint8_t *stage = epi + (group * 2 + buf) * kRowBuf;
+            __nv_bfloat16 *col = reinterpret_cast<__nv_bfloat16 *>(stage) + quad * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < kChunkRows; i++) col[i * (kRowPitch / 2)] = __float2bfloat16(value(i));
+            epi_bar(group);
+            const int first = c * kChunkRows;
+            const int64_t row0 = (int64_t)w.row0 + w.n0 + group * kHalf + first;
+            __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + row0 * m_size + m_first;
+#pragma unroll
+            for (int q = 0; q < kChunkRows / 8; q++) {
+                const int r = q * 8 + (et >> 4), seg = et & 15;
+                if (first + r < left && m_first + seg * 8 < m_size)
+                    *reinterpret_cast<uint4 *>(out + (int64_t)r * m_size + seg * 8) =
+                        *reinterpret_cast<const uint4 *>(stage + r * kRowPitch + seg * 16);
+            }
+            buf ^= 1;  // the next chunk's barrier separates this buffer's reads from its next writes
+        };
         for (int64_t u = cluster; u < total; u += n_clusters) {
             const Unit w = units.at(u);
             const int m_first = w.m0 + (int)rank * kHalf;
             const int left = w.n_valid - group * kHalf;  // columns for this group
-            if (OP != kWeightGrad) {
+            if constexpr (OP != kWeightGrad && RUNS) {
+                float sum[kHalf];
+                if (!add_runs(w, left, sum)) break;
+#pragma unroll
+                for (int c = 0; c < kHalf / kChunkRows; c++)
+                    if (c * kChunkRows < left)
+                        store_rows(w, c, m_first, left, [&](int i) { return sum[c * kChunkRows + i]; });
+            } else if constexpr (OP != kWeightGrad) {
                 const uint32_t acc = run & 1;
                 const bool ready = wait_for(&tmem_full[acc], (run >> 1) & 1, ab, 4);
                 if (!epi_vote(group, ready)) break;
@@ -478,48 +552,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld16(t_warp + acc * kTileN + c * kChunkRows, v);
                     tmem_ld_wait();
                     if (c == chunks - 1) release(acc);
-                    uint8_t *stage = epi + (group * 2 + buf) * kRowBuf;
-                    __nv_bfloat16 *col = reinterpret_cast<__nv_bfloat16 *>(stage) + quad * 32 + lane;
-#pragma unroll
-                    for (int i = 0; i < kChunkRows; i++)
-                        col[i * (kRowPitch / 2)] = __float2bfloat16(__uint_as_float(v[i]));
-                    epi_bar(group);
-                    const int first = c * kChunkRows;
-                    const int64_t row0 = (int64_t)w.row0 + w.n0 + group * kHalf + first;
-                    __nv_bfloat16 *out = (__nv_bfloat16 *)a.out + row0 * m_size + m_first;
-#pragma unroll
-                    for (int q = 0; q < kChunkRows / 8; q++) {
-                        const int r = q * 8 + (et >> 4), seg = et & 15;
-                        if (first + r < left && m_first + seg * 8 < m_size)
-                            *reinterpret_cast<uint4 *>(out + (int64_t)r * m_size + seg * 8) =
-                                *reinterpret_cast<const uint4 *>(stage + r * kRowPitch + seg * 16);
-                    }
-                    buf ^= 1;  // the next chunk's barrier separates this buffer's reads from its next writes
+                    store_rows(w, c, m_first, left, [&](int i) { return __uint_as_float(v[i]); });
                 }
             } else {
-                // lanes are rows of dW; the runs' sums in registers
-                const int run_stages = run_stages_of<OP>(a, w);
+                // lanes are rows of dW
                 float sum[kHalf];
-#pragma unroll
-                for (int i = 0; i < kHalf; i++) sum[i] = 0.f;
-                bool ok = true;
-                for (int s0 = 0; s0 < w.stages; s0 += run_stages, run++) {
-                    const uint32_t acc = run & 1;
-                    const bool ready = wait_for(&tmem_full[acc], (run >> 1) & 1, ab, 4);
-                    if (!(ok = epi_vote(group, ready))) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < kHalf / 16; c++)
-                        if (c * 16 < left) {
-                            uint32_t v[16];
-                            tmem_ld16(t_warp + acc * kTileN + c * 16, v);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; i++) sum[c * 16 + i] += __uint_as_float(v[i]);
-                        }
-                    release(acc);
-                }
-                if (!ok) break;
+                if (!add_runs(w, left, sum)) break;
                 const bool f32 = a.out_f32 || w.part >= 0, add = a.accumulate && w.part < 0;
                 if (!add) {
                     // TMA writes the rows out, and leaves out what lies past the last row and column: the LSU path
@@ -684,8 +722,8 @@ View chunks(int64_t rows, int64_t cols) {
 int part_rows(int64_t rows, int64_t inputs, int64_t outputs, int groups) {
     const int64_t area = ((outputs + kTileM - 1) / kTileM) * ((inputs + kTileN - 1) / kTileN);
     if (area * groups >= 74 || rows < (int64_t)groups * 2048) return kAnyRows;
-    const int64_t run = kRunStages * kStageK, want = (rows * area / 148 + run - 1) / run * run;
-    return (int)(want < run ? run : want);
+    const int64_t want = (rows * area / 148 + kPartStep - 1) / kPartStep * kPartStep;
+    return (int)(want < kPartStep ? kPartStep : want);
 }
 
 // Adds the parts' sums of every group that was split, in order, four values
@@ -725,9 +763,9 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const DenseArgs a) {
     }
 }
 
-template <GroupedOp OP>
+template <GroupedOp OP, bool RUNS>
 int launch(const GroupedProduct &p, int device, cudaStream_t st) {
-    auto kern = grouped_dense_kernel<OP>;
+    auto kern = grouped_dense_kernel<OP, RUNS>;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmemBytes;
@@ -817,15 +855,16 @@ bool grouped_dense_usable(const GroupedProduct &p) {
     // TMA: rows and bases on 16 bytes; the epilogue stores 16 bytes.  A sum
     // over no rows at all has nothing to map.  A launch's tiles are counted in 31 bits.
     const int64_t m_tiles = (p.outputs + kTileM - 1) / kTileM, n_tiles = (p.inputs + kTileN - 1) / kTileN;
-    const int64_t terms = p.op == kProduct ? p.inputs : p.op == kInputGrad ? p.outputs : 0;
-    return p.dtype == GTMOE_DTYPE_BF16 && p.rows > 0 && terms <= kMostSumTerms && p.inputs % 8 == 0 && p.outputs % 8 == 0 && aligned16(p.a) &&
+    return p.dtype == GTMOE_DTYPE_BF16 && p.rows > 0 && p.inputs % 8 == 0 && p.outputs % 8 == 0 && aligned16(p.a) &&
            aligned16(p.b) && aligned16(p.c) && m_tiles * n_tiles < 0x7ffffffe / p.groups;
 }
 
 int launch_grouped_dense(const GroupedProduct &p, int device, cudaStream_t st) {
-    if (p.op == kProduct) return launch<kProduct>(p, device, st);
-    if (p.op == kInputGrad) return launch<kInputGrad>(p, device, st);
-    return launch<kWeightGrad>(p, device, st);
+    if (p.op == kWeightGrad) return launch<kWeightGrad, true>(p, device, st);
+    const int64_t terms = p.op == kProduct ? p.inputs : p.outputs;
+    if (terms > kLongRunStages * kStageK)
+        return p.op == kProduct ? launch<kProduct, true>(p, device, st) : launch<kInputGrad, true>(p, device, st);
+    return p.op == kProduct ? launch<kProduct, false>(p, device, st) : launch<kInputGrad, false>(p, device, st);
 }
 
 int64_t grouped_dense_workspace(int64_t rows, int64_t inputs, int64_t outputs, int groups) {

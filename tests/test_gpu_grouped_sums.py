@@ -1,0 +1,117 @@
+"""Long sums of the grouped products: how many terms there are, and whether
+they have one sign or repeat, may not show beyond each result's own precision.
+
+The tensor cores cut additions towards zero (at most 2^-23 of the sum each),
+so a sum is made in runs of stages of 64 terms, four additions to a stage: 8
+stages for float32 results, 128 for bfloat16 ones.  Runs are added with
+rounding, and what sixteen of them round off is carried along, so the bounds
+below are those of a run."""
+import pytest
+import torch
+
+import operators_ref as R
+from gotransformers_b200 import moe
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def device_counts(counts):
+    return torch.tensor(counts, dtype=torch.int64, device="cuda")
+
+
+def spread(rows, columns, seed, scaled):
+    """Positive values with a factor of their own, between 1 and 2, per row or
+    per column, so that sums over the other axis fall anywhere between two
+    bfloat16 numbers."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    v = 0.75 + 0.5 * torch.rand(rows, columns, generator=g, device="cuda")
+    f = 1 + torch.rand((rows, 1) if scaled == "rows" else (1, columns), generator=g, device="cuda")
+    return (v * f).to(BF16)
+
+
+def lean(got, ref):
+    """The mean relative error: where it points."""
+    return float(((got.double() - ref) / ref).mean())
+
+
+@pytest.mark.parametrize("call", ["product", "input gradients", "weight gradients"])
+def test_bfloat16_results_do_not_lean(call):
+    """65536 results, each a sum of many terms of one sign.  Roundings to
+    bfloat16 err evenly to both sides, at most 2^-8 each with a deviation of at
+    most 2^-8 / sqrt(3): the mean of 256 x 256 of them whose 256 row factors
+    and 256 column factors are independent is within 8 deviations / 256.  The
+    cut additions of a run are at most 512 * 2^-23, half of that on average for
+    an even cut and half again because partial sums grow evenly; one sum over
+    all the terms would lean by 1.6e-3 (262144 terms)."""
+    n = 1 << 18 if call != "weight gradients" else 60000
+    if call == "weight gradients":
+        x, dy = spread(n, 256, 1, "columns"), spread(n, 256, 2, "columns")
+        ref = dy.double().T @ x.double()
+        # 80 groups: no group's rows are split
+        got = moe.grouped_product_weight_gradients(dy, x, device_counts([n] + [0] * 79))[0]
+    else:
+        x, w = spread(256, n, 3, "rows"), spread(256, n, 4, "rows")
+        ref = x.double() @ w.double().T
+        c = device_counts([256])
+        if call == "product":
+            got = moe.grouped_product(x, w[None], c)
+        else:
+            got = moe.grouped_product_input_gradients(x, w.T.contiguous()[None], c)
+    assert abs(lean(got, ref)) <= 8 * 2.0**-8 / 3**0.5 / 256 + 512 * 2.0**-23 / 4
+    R.within("results", got, ref.cpu(), ref.cpu().abs() * (R.HALF[BF16] + (512 + 33) * 2.0**-23))
+    moe.check_operators()
+
+
+@pytest.mark.parametrize("inputs,outputs,counts", [
+    (8200, 72, [70, 0, 300]), (72, 8200, [70, 0, 300]), (16384, 264, [1, 257]), (264, 20000, [33, 128, 95]),
+    (140000, 40, [5, 20]), (40, 140000, [5, 20]),
+])
+def test_products_over_many_terms_are_exact_on_whole_numbers(inputs, outputs, counts):
+    """More than one run, and more runs than are kept in registers."""
+    g = torch.Generator().manual_seed(inputs)
+    rows, groups = sum(counts) + 3, len(counts)
+    x = torch.randint(-4, 5, (rows, inputs), generator=g).to(BF16)
+    w = torch.randint(-4, 5, (groups, outputs, inputs), generator=g).to(BF16)
+    dy = torch.randint(-4, 5, (rows, outputs), generator=g).to(BF16)
+    x[-3:], dy[-3:] = float("nan"), float("nan")
+    n, C = rows - 3, device_counts(counts)
+    y = torch.full((rows, outputs), 7.0, dtype=BF16, device="cuda")
+    dx = torch.full((rows, inputs), 7.0, dtype=BF16, device="cuda")
+    moe.grouped_product(x.cuda(), w.cuda(), C, out=y)
+    moe.grouped_product_input_gradients(dy.cuda(), w.cuda(), C, input_gradients=dx)
+    assert torch.equal(y[:n].cpu(), R.grouped(x[:n], w, counts).to(BF16))
+    assert torch.equal(dx[:n].cpu(), R.grouped_input_gradients(dy[:n], w, counts).to(BF16))
+    assert (y[n:] == 7).all() and (dx[n:] == 7).all()
+    moe.check_operators()
+
+
+@pytest.mark.parametrize("groups", [80, 1])
+def test_float32_weight_gradients_of_constant_rows(groups):
+    """16.8 million equal rows.  A run's sums are exact here, and where the
+    runs' sum rounds, it rounds the same way again and again: 1.6e-4 of it if
+    they were added one by one.  Carried along, at most the 2^-24 of 16 runs
+    and of the last addition are left; a group that is split has at most 148
+    parts, added one by one."""
+    n = (1 << 24) + 37
+    x = torch.full((n, 8), 171 / 128, dtype=BF16, device="cuda")
+    dw = moe.grouped_product_weight_gradients(x, x, device_counts([n] + [0] * (groups - 1)), dtype=F32)[0]
+    ref = n * (171 / 128) ** 2
+    tol = 17 * 2.0**-24 + (148 * 2.0**-24 if groups == 1 else 0)
+    assert float((dw.double() / ref - 1).abs().max()) <= tol
+    moe.check_operators()
+
+
+@pytest.mark.parametrize("groups", [80, 1])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_infinite_sums_stay_infinite(groups, dtype):
+    n = 40000
+    x, dy = spread(n, 64, 5, "columns"), spread(n, 64, 6, "columns")
+    x[100, 3], x[39999, 7], x[20000, 9], x[5, 11] = float("inf"), float("inf"), float("nan"), -float("inf")
+    dw = moe.grouped_product_weight_gradients(dy, x, device_counts([n] + [0] * (groups - 1)), dtype=dtype)[0].cpu()
+    inf = torch.full((64,), float("inf"), dtype=dtype)
+    assert torch.equal(dw[:, 3], inf) and torch.equal(dw[:, 7], inf) and torch.equal(dw[:, 11], -inf)
+    assert torch.isnan(dw[:, 9]).all()
+    rest = [c for c in range(64) if c not in (3, 7, 9, 11)]
+    assert torch.isfinite(dw[:, rest]).all()
