@@ -469,9 +469,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // this warp's part of a unit's D, its runs added up with rounding; false when a wait gave up
         auto add_runs = [&](const Unit &w, int left, float (&sum)[kHalf]) {
             const int run_stages = run_stages_of<OP, RUNS>(a, w);
-            float folded[kHalf];  // in local memory, which units of at most kFoldRuns runs do not touch
-            int at = 0, runs = 0;
-            asm volatile("" : "+r"(at));
+            // in local memory, which units of at most kFoldRuns runs do not touch: at is 0, but the compiler does not see
+            // that and so keeps the registers for the sums
+            float folded[kHalf];
+            const int at = (int)(a.rows >> 40);
+            int runs = 0;
 #pragma unroll
             for (int i = 0; i < kHalf; i++) sum[i] = 0.f;
             for (int s0 = 0; s0 < w.stages; s0 += run_stages, run++, runs++) {
