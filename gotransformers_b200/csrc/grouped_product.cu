@@ -10,6 +10,8 @@ namespace {
 __device__ int g_error;  // first code a kernel recorded since the last check
 
 constexpr int kThreads = 256;
+constexpr int kRunTerms = 256;      // terms of a long float32 sum per run
+constexpr int kOneRunTerms = 1024;  // and how many a sum may have that is made in one
 
 // One operand of a tile: TILE values along the tile's axis by STEP terms.
 // KMAJOR: the terms are contiguous in memory, else the tile's axis is.
@@ -58,11 +60,16 @@ struct Operand {
 //   kInputGrad   i row, j input,  p output:  A = dY[i][p], B = W_g[p][j]
 //   kWeightGrad  i output, j input, p row:   A = dY[p][i], B = X[p][j]
 // TI x TJ outputs per block, (TI / 16) x (TJ / 16) per thread, each one sum in
-// ascending p in ACC, STEP terms per shared-memory step.  Two buffers: one
-// barrier per step.  FFMA-bound: 16384 rows in 8 groups, 1024 x 1024, float32
+// ascending p, STEP terms per shared-memory step.  Two buffers: one barrier per
+// step.  RUNS: a long float32 sum is made in runs of kRunTerms terms, which join
+// a total in local memory, and what that addition rounds off is carried on
+// (fold()).  One sum was off by 2.1e-5 after 1536 equal terms, 5.9e-5 after
+// 65536, and stopped growing at 2^24 ones.  The runs take 7 % more time at most
+// (4096 rows in 8 groups, 4096 -> 1024: 842 -> 891 us; weight gradient of 16384
+// rows in 8 groups, 1024 x 1024: 927 -> 910 us).  FFMA-bound: 16384 rows in 8 groups, 1024 x 1024, float32
 // 45 TF/s (cuBLAS's float32 product of this size of sums 57).
-template <typename T, typename ACC, typename OUT, GroupedOp OP, int TI, int TJ, int STEP>
-__global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const GroupedProduct a) {
+template <typename T, typename ACC, typename OUT, GroupedOp OP, bool RUNS, int TI, int TJ, int STEP>
+__global__ void __launch_bounds__(kThreads, TI == 128 && RUNS ? 2 : 0) grouped_simt_product_kernel(const GroupedProduct a) {
     // outputs per thread and axis, in runs of VI and VJ
     constexpr int RI = TI / 16, VI = RI < 4 ? RI : 4, RJ = TJ / 16, VJ = RJ < 4 ? RJ : 4;
     __shared__ __align__(16) ACC sa[2][STEP][TI + 4], sb[2][STEP][TJ + 4];
@@ -95,6 +102,10 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
         ACC acc[RI][RJ] = {};
         oa.load(0);
         ob.load(0);
+        // in local memory, which sums of one run do not touch: at is 0, but the compiler does not see that and so
+        // keeps the registers for the products
+        float total[RI * RJ];
+        const int at = (int)(a.rows >> 40);
         int buf = 0;
         for (int64_t p0 = 0; p0 < p_end; p0 += STEP, buf ^= 1) {
             oa.store(sa[buf]);
@@ -116,7 +127,25 @@ __global__ void __launch_bounds__(kThreads) grouped_simt_product_kernel(const Gr
 #pragma unroll
                     for (int y = 0; y < RJ; y++) acc[x][y] += ra[x] * rb[y];
             }
+            if constexpr (RUNS)
+                if ((p0 + STEP) % kRunTerms == 0 && p0 + STEP < p_end) {
+                    const bool first = p0 + STEP == kRunTerms;
+#pragma unroll
+                    for (int x = 0; x < RI; x++)
+#pragma unroll
+                        for (int y = 0; y < RJ; y++) {
+                            float &t = total[at + x * RJ + y];
+                            if (first) t = 0.f;
+                            fold(t, acc[x][y]);
+                        }
+                }
         }
+        if constexpr (RUNS)
+            if (p_end > kRunTerms)
+#pragma unroll
+                for (int x = 0; x < RI; x++)
+#pragma unroll
+                    for (int y = 0; y < RJ; y++) acc[x][y] += total[at + x * RJ + y];
         __syncthreads();  // the buffers are free for the next tile
         OUT *C = (OUT *)a.c;
         const int64_t base = OP == kWeightGrad ? (int64_t)g * a.outputs * a.inputs : r0 * n_j;
@@ -142,11 +171,11 @@ int64_t most_tiles(const GroupedProduct &p, int ti, int tj) {
     return i_tiles * ((n_j + tj - 1) / tj);
 }
 
-template <typename T, typename ACC, typename OUT, GroupedOp OP, int TI, int TJ, int STEP>
+template <typename T, typename ACC, typename OUT, GroupedOp OP, bool RUNS, int TI, int TJ, int STEP>
 int launch_simt_tile(const GroupedProduct &p, cudaStream_t st) {
     const int64_t most = most_tiles<OP>(p, TI, TJ);
     const unsigned grid = (unsigned)(most < 148 * 16 ? most : 148 * 16);
-    grouped_simt_product_kernel<T, ACC, OUT, OP, TI, TJ, STEP><<<grid, kThreads, 0, st>>>(p);
+    grouped_simt_product_kernel<T, ACC, OUT, OP, RUNS, TI, TJ, STEP><<<grid, kThreads, 0, st>>>(p);
     GT_CUDA(cudaGetLastError());
     note_launches(1);
     return 0;
@@ -157,16 +186,25 @@ int launch_simt_tile(const GroupedProduct &p, cudaStream_t st) {
 // of 128 x 128 (64 products per 16 values read) once they are enough for every
 // SM and the groups fill them, else of 64 x 64; float64 has shared memory for
 // the latter only.
-template <typename T, typename ACC, typename OUT, GroupedOp OP>
-int launch_simt(const GroupedProduct &p, cudaStream_t st) {
+template <typename T, typename ACC, typename OUT, GroupedOp OP, bool RUNS>
+int launch_simt_tiles(const GroupedProduct &p, cudaStream_t st) {
     if constexpr (sizeof(ACC) == 4) {
         const int64_t average = p.rows / p.groups;
         if constexpr (OP != kWeightGrad)
-            if (average < 48) return launch_simt_tile<T, ACC, OUT, OP, 32, 64, 32>(p, st);
+            if (average < 48) return launch_simt_tile<T, ACC, OUT, OP, RUNS, 32, 64, 32>(p, st);
         if ((OP == kWeightGrad || average >= 96) && most_tiles<OP>(p, 128, 128) >= 2 * 148)
-            return launch_simt_tile<T, ACC, OUT, OP, 128, 128, 16>(p, st);
+            return launch_simt_tile<T, ACC, OUT, OP, RUNS, 128, 128, 16>(p, st);
     }
-    return launch_simt_tile<T, ACC, OUT, OP, 64, 64, 16>(p, st);
+    return launch_simt_tile<T, ACC, OUT, OP, RUNS, 64, 64, 16>(p, st);
+}
+
+// Float32 sums that may have more than kOneRunTerms terms are made in runs.
+template <typename T, typename ACC, typename OUT, GroupedOp OP>
+int launch_simt(const GroupedProduct &p, cudaStream_t st) {
+    if constexpr (sizeof(ACC) == 4)
+        if ((OP == kProduct ? p.inputs : OP == kInputGrad ? p.outputs : p.rows) > kOneRunTerms)
+            return launch_simt_tiles<T, ACC, OUT, OP, true>(p, st);
+    return launch_simt_tiles<T, ACC, OUT, OP, false>(p, st);
 }
 
 template <typename T, typename ACC>

@@ -5,7 +5,8 @@ The tensor cores cut additions towards zero (at most 2^-23 of the sum each),
 so a sum is made in runs of stages of 64 terms, four additions to a stage: 8
 stages for float32 results, 128 for bfloat16 ones.  Runs are added with
 rounding, and what sixteen of them round off is carried along, so the bounds
-below are those of a run."""
+below are those of a run.  The SIMT cores make sums of more than 1024 terms in
+runs of 256 rounded additions and carry what every run's addition rounds off."""
 import pytest
 import torch
 
@@ -114,4 +115,65 @@ def test_infinite_sums_stay_infinite(groups, dtype):
     assert torch.equal(dw[:, 3], inf) and torch.equal(dw[:, 7], inf) and torch.equal(dw[:, 11], -inf)
     assert torch.isnan(dw[:, 9]).all()
     rest = [c for c in range(64) if c not in (3, 7, 9, 11)]
+    assert torch.isfinite(dw[:, rest]).all()
+
+
+@pytest.mark.parametrize("value,n", [(1.0, (1 << 25) + 37), (171 / 128, (1 << 22) + 37)])
+@pytest.mark.parametrize("dtype,width,wdtype", [(F32, 8, F32), (BF16, 7, F32), (BF16, 7, BF16)])
+def test_equal_rows_on_the_simt_cores(value, n, dtype, width, wdtype):
+    """Float32 operands, and bfloat16 ones that the tensor cores cannot
+    address.  One float32 sum stops growing at 2^24 ones, and rounds equal
+    values alike again and again.  A run's partial sums grow evenly, so its 256
+    additions err by at most 129 * 2^-24 of it; what is carried along can make
+    each err by 2^-24 of 2^-24 of the total."""
+    x = torch.full((n, width), value, dtype=dtype, device="cuda")
+    dw = moe.grouped_product_weight_gradients(x, x, device_counts([n]), dtype=wdtype)[0]
+    ref = n * value * value
+    half = R.HALF[BF16] if wdtype == BF16 else 0
+    assert float((dw.double() / ref - 1).abs().max()) <= half + 131 * 2.0**-24 + n * 2.0**-48
+
+
+@pytest.mark.parametrize("value", [1.0, 171 / 128])
+@pytest.mark.parametrize("call", ["product", "input gradients"])
+def test_equal_terms_on_the_simt_cores(value, call):
+    n = (1 << 24) + 4099
+    x = torch.full((3, n), value, device="cuda")
+    if call == "product":
+        y = moe.grouped_product(x, x[:2].view(1, 2, n), device_counts([3]))
+    else:
+        y = moe.grouped_product_input_gradients(x, x[:2].reshape(1, n, 2), device_counts([3]))
+    ref = n * value * value
+    assert float((y.double() / ref - 1).abs().max()) <= 131 * 2.0**-24 + n * 2.0**-48
+
+
+@pytest.mark.parametrize("n", [255, 257, 512, 513, 768, 1024, 1025, 1280, 1300])
+@pytest.mark.parametrize("inputs,outputs", [(20, 24), (200, 130)])
+def test_runs_on_the_simt_cores_are_exact_on_whole_numbers(n, inputs, outputs):
+    """Terms around a run's end, in each direction and tile, added to what is there too."""
+    g = torch.Generator().manual_seed(n)
+
+    def whole(*s):
+        return torch.randint(-4, 5, s, generator=g).float()
+
+    for rows, k, m, counts in ((9, n, outputs, [4, 5]), (300, n, outputs, [300]), (9, inputs, n, [4, 5]),
+                               (300, inputs, n, [300]), (2 * n, inputs, outputs, [n, n])):
+        x, w, dy, C = whole(rows, k), whole(len(counts), m, k), whole(rows, m), device_counts(counts)
+        assert torch.equal(moe.grouped_product(x.cuda(), w.cuda(), C).cpu(), R.grouped(x, w, counts).float())
+        dx = moe.grouped_product_input_gradients(dy.cuda(), w.cuda(), C).cpu()
+        assert torch.equal(dx, R.grouped_input_gradients(dy, w, counts).float())
+        dw = w.cuda()
+        moe.grouped_product_weight_gradients(dy.cuda(), x.cuda(), C, weight_grad=dw)
+        assert torch.equal(dw.cpu(), (R.grouped_weight_gradients(dy, x, counts) + w.double()).float())
+    moe.check_operators()
+
+
+def test_infinite_sums_on_the_simt_cores_stay_infinite():
+    n = 5000
+    x, dy = spread(n, 63, 5, "columns").float(), spread(n, 65, 6, "columns").float()
+    x[100, 3], x[4999, 7], x[2000, 9], x[5, 11] = float("inf"), float("inf"), float("nan"), -float("inf")
+    dw = moe.grouped_product_weight_gradients(dy, x, device_counts([n]))[0].cpu()
+    inf = torch.full((65,), float("inf"))
+    assert torch.equal(dw[:, 3], inf) and torch.equal(dw[:, 7], inf) and torch.equal(dw[:, 11], -inf)
+    assert torch.isnan(dw[:, 9]).all()
+    rest = [c for c in range(63) if c not in (3, 7, 9, 11)]
     assert torch.isfinite(dw[:, rest]).all()
