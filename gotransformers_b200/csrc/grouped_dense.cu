@@ -200,14 +200,22 @@ struct Aborts {
     volatile int *own;
     uint32_t peer;
 };
-// Bounded wait with cluster-scope acquire; false when it gave up.
-__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, const Aborts &ab, int code) {
+// Bounded wait with cluster-scope acquire; false when it gave up.  progress: a
+// count that others move before the barrier's turn comes; the limit runs from
+// its last change.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, const Aborts &ab, int code,
+                                         const volatile uint32_t *progress = nullptr) {
     if (mbar_try_wait_cluster(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
+    uint32_t seen = progress ? *progress : 0;
+    uint64_t t0 = global_timer_ns();
     while (true) {
         for (int i = 0; i < 32; i++)
             if (mbar_try_wait_cluster(bar, parity)) return true;
         if (*ab.own) return false;
+        if (progress && *progress != seen) {
+            seen = *progress;
+            t0 = global_timer_ns();
+        }
         if (global_timer_ns() - t0 > kWaitLimitNs) {
             atomicCAS(&g_dense_error, 0, code);
             *ab.own = 1;
@@ -305,7 +313,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *tmem_full = bars + 3 * kStages; // [2] accumulator ready (both CTAs)
     uint64_t *tmem_empty = tmem_full + 2;     // [2] both epilogues done (leader)
     uint32_t *tmem_slot = (uint32_t *)(tmem_full + 4);
-    static_assert((3 * kStages + 4) * 8 + 8 <= kBarBytes, "barrier area");
+    volatile uint32_t *loaded = tmem_slot + 2;  // stages that the warp that loads A has issued
+    static_assert((3 * kStages + 4) * 8 + 12 <= kBarBytes, "barrier area");
     int *start = (int *)((uint8_t *)bars + kBarBytes);
     int *tiles = start + kMaxGroups + 1;
     int *scratch = tiles + kMaxGroups + 1;
@@ -330,6 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&tmem_empty[b], 2 * kEpiWarps);
         }
         *ab.own = 0;
+        *loaded = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -412,6 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         else tma_pair(sa + i * kChunkBytes, &maps.a_edge, am + 64 * i, w.row0 + k0, bar);
                     }
                 }
+                if (OP == kWeightGrad && loads_a && issuer) *loaded = j + 1;
                 __syncwarp();
             }
         }
@@ -657,7 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             j += w.stages;
             if (w.stages == 0 || valid == 0) continue;
             const int sb = (int)((j - 1) % kStages);
-            ok = wait_for(&tail[sb], (phases >> sb) & 1, ab, 5);
+            // from here on the ring may go around millions of times before that stage's turn
+            ok = wait_for(&tail[sb], (phases >> sb) & 1, ab, 5, loaded);
             phases ^= 1u << sb;
             if (!__all_sync(0xffffffffu, ok)) break;
             uint8_t *tile = smem + sb * kStageBytes;

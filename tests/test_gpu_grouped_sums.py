@@ -177,3 +177,19 @@ def test_infinite_sums_on_the_simt_cores_stay_infinite():
     assert torch.isnan(dw[:, 9]).all()
     rest = [c for c in range(63) if c not in (3, 7, 9, 11)]
     assert torch.isfinite(dw[:, rest]).all()
+
+
+def test_a_row_tail_after_seconds_of_whole_stages():
+    """80 groups are not split: one pair of SMs takes 700 million rows by
+    itself, 280 ns per 64 of them and three seconds in all, before it gets to
+    the stage that the group's last 37 rows do not fill.  What waits for that
+    stage may not give up after two."""
+    n = 700_000_037
+    x = torch.ones(n, 8, dtype=BF16, device="cuda")
+    x[-1] = 4096.0
+    moe.check_operators()
+    dw = moe.grouped_product_weight_gradients(x, x, device_counts([0] * 79 + [n]), dtype=F32)
+    moe.check_operators()
+    assert not dw[:-1].any()
+    ref = n - 1 + 4096.0**2
+    assert float((dw[-1].double() / ref - 1).abs().max()) <= 17 * 2.0**-24
