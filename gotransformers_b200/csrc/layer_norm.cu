@@ -806,7 +806,9 @@ int gtmoe_layer_norm(const void *x, int dtype, int64_t rows, int64_t width, cons
     if (overlaps_shifted(x, bytes, y, bytes) || ranges_overlap(weight, pbytes, y, bytes) ||
         ranges_overlap(bias, pbytes, y, bytes) || ranges_overlap(mean, sbytes, y, bytes) ||
         ranges_overlap(rstd, sbytes, y, bytes) || ranges_overlap(mean, sbytes, x, bytes) ||
-        ranges_overlap(rstd, sbytes, x, bytes) || ranges_overlap(mean, sbytes, rstd, sbytes))
+        ranges_overlap(rstd, sbytes, x, bytes) || ranges_overlap(mean, sbytes, rstd, sbytes) ||
+        ranges_overlap(mean, sbytes, weight, pbytes) || ranges_overlap(mean, sbytes, bias, pbytes) ||
+        ranges_overlap(rstd, sbytes, weight, pbytes) || ranges_overlap(rstd, sbytes, bias, pbytes))
         return fail(GTMOE_EINVAL, "layer norm: an output overlaps another argument (y may be x itself)");
     DeviceScope scope;
     const size_t es = dtype_size(dtype), ws = dtype_size(weight_dtype), ss = dtype == GTMOE_DTYPE_F64 ? 8 : 4;
