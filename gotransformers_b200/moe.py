@@ -21,6 +21,8 @@ import numpy as np
 from . import _lib
 from ._lib import DOWN, DTYPE_BF16, DTYPE_F32, DTYPE_F64, FLOAT32, FLOAT64, FP4, GATE, INT8, ROUTED, SHARED, UP, check
 from .operators import (
+    _generator,
+    _number,
     check_operators,
     dropout,
     dropout_backward,
@@ -289,7 +291,8 @@ class MixtureOfExperts:
         """Dropout of the mixture's output inside forward_block: x +
         dropout(Forward(RMSNorm(x))) from now on, with dropout()'s decisions
         for (rate, seed, stream); rate 0 switches it off."""
-        check(_lib.lib().gtmoe_set_dropout(self._h, float(rate), seed, stream))
+        seed, stream, _ = _generator(seed, stream)
+        check(_lib.lib().gtmoe_set_dropout(self._h, _number("rate", rate), seed, stream))
 
     # -- training
     def set_training(self, on: bool = True):

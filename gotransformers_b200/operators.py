@@ -10,6 +10,7 @@ graph: the gradients are the functions named so.  Misuse raises
 from __future__ import annotations
 
 import ctypes
+import numbers
 
 from . import _lib
 from ._lib import DTYPE_BF16, DTYPE_F32, DTYPE_F64, check
@@ -86,6 +87,28 @@ def _stream(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def _number(name: str, v):
+    if type(v) is not float:
+        if not isinstance(v, numbers.Real):
+            raise ValueError(f"{name} must be a number, got {type(v).__name__}")
+        v = float(v)
+    return v
+
+
+def _generator(seed, stream, offset=0):
+    """The generator's arguments; of longer ones the library would see the last 64 bits."""
+    out = []
+    for name, v, end in (("seed", seed, 1 << 64), ("stream", stream, 1 << 64), ("offset", offset, 1 << 63)):
+        if type(v) is not int:
+            if not isinstance(v, numbers.Integral):
+                raise ValueError(f"{name} must be a whole number, got {type(v).__name__}")
+            v = int(v)
+        if not -(1 << 63) <= v < end:
+            raise ValueError(f"{name} must be a number of 64 bits, got {v}")
+        out.append(v)
+    return out
+
+
 def _dtype(a):
     """a's dtype; None for what is no tensor, which the checks then refuse."""
     return getattr(a, "dtype", None)
@@ -116,8 +139,8 @@ def layer_norm(x, weight=None, bias=None, epsilon: float = 1e-6, out=None):
         po = _tensor("out", out, shape, dtype, dev)
     mean = torch.empty(rows, dtype=_stats_dtype(x), device=x.device)
     rstd = torch.empty_like(mean)
-    check(_L.gtmoe_layer_norm(px, code, rows, width, pw, pb, wcode, epsilon, po, mean.data_ptr(), rstd.data_ptr(),
-                              _stream(dev)))
+    check(_L.gtmoe_layer_norm(px, code, rows, width, pw, pb, wcode, _number("epsilon", epsilon), po, mean.data_ptr(),
+                              rstd.data_ptr(), _stream(dev)))
     return out, mean, rstd
 
 
@@ -186,7 +209,8 @@ def dropout(x, rate: float, seed: int, stream: int = 0, offset: int = 0, residua
         po = out.data_ptr()
     else:
         po = _tensor("out", out, shape, dtype, dev)
-    check(_L.gtmoe_dropout(px, pr, code, x.numel(), rate, seed, stream, offset, po, _stream(dev)))
+    check(_L.gtmoe_dropout(px, pr, code, x.numel(), _number("rate", rate), *_generator(seed, stream, offset), po,
+                           _stream(dev)))
     return out
 
 
@@ -203,7 +227,8 @@ def dropout_backward(output_gradients, rate: float, seed: int, stream: int = 0, 
         pdx = input_gradients.data_ptr()
     else:
         pdx = _tensor("input_gradients", input_gradients, g.shape, g.dtype, dev)
-    check(_L.gtmoe_dropout_backward(pg, code, g.numel(), rate, seed, stream, offset, pdx, _stream(dev)))
+    check(_L.gtmoe_dropout_backward(pg, code, g.numel(), _number("rate", rate), *_generator(seed, stream, offset),
+                                    pdx, _stream(dev)))
     return input_gradients
 
 
