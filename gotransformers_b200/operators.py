@@ -5,7 +5,8 @@ expert, each with its gradients (the last section of include/gtmoe.h).
 Arguments are CUDA tensors of one device, contiguous, float64, float32 or
 bfloat16; a call runs on that device's current torch stream, waits for
 nothing and may be captured into a CUDA graph.  Results carry no autograd
-graph: the gradients are the functions named so.  Misuse raises
+graph: the gradients are the functions named so; a tensor that a call was given
+to write into counts as changed for autograd.  Misuse raises
 ``ValueError``, what the library refuses ``GtmoeError``."""
 from __future__ import annotations
 
@@ -109,6 +110,14 @@ def _generator(seed, stream, offset=0):
     return out
 
 
+def _wrote(*given):
+    """The library writes through addresses: tells autograd that the caller's
+    tensors have changed, so that it refuses to use what it had saved of them."""
+    for t in given:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _dtype(a):
     """a's dtype; None for what is no tensor, which the checks then refuse."""
     return getattr(a, "dtype", None)
@@ -132,6 +141,7 @@ def layer_norm(x, weight=None, bias=None, epsilon: float = 1e-6, out=None):
     pw = None if weight is None else _tensor("weight", weight, (width,), wdt, dev)
     pb = None if bias is None else _tensor("bias", bias, (width,), wdt, dev)
     code, wcode = _code(dtype), _code(wdt)
+    given = out
     if out is None:
         out = torch.empty_like(x)
         po = out.data_ptr()
@@ -141,6 +151,8 @@ def layer_norm(x, weight=None, bias=None, epsilon: float = 1e-6, out=None):
     rstd = torch.empty_like(mean)
     check(_L.gtmoe_layer_norm(px, code, rows, width, pw, pb, wcode, _number("epsilon", epsilon), po, mean.data_ptr(),
                               rstd.data_ptr(), _stream(dev)))
+    if given is not None:
+        _wrote(given)
     return out, mean, rstd
 
 
@@ -166,6 +178,7 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
     pres = None
     if residual_gradients is not None:
         pres = _tensor("residual_gradients", residual_gradients, shape, dtype, dev)
+    given = input_gradients
     if input_gradients is None:
         input_gradients = torch.empty_like(g)
         pdx = input_gradients.data_ptr()
@@ -192,6 +205,8 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
         pwork = work.data_ptr()
     check(_L.gtmoe_layer_norm_backward(pg, px, code, rows, width, pw, wcode, pm, pr, pres, pdx, pdw, pdb,
                                        int(accumulate), pwork, nbytes, _stream(dev)))
+    if given is not None or accumulate:
+        _wrote(given, *((weight_grad, bias_grad) if accumulate else ()))
     return input_gradients, weight_grad, bias_grad
 
 
@@ -204,6 +219,7 @@ def dropout(x, rate: float, seed: int, stream: int = 0, offset: int = 0, residua
     shape, dtype = x.shape, x.dtype
     pr = None if residual is None else _tensor("residual", residual, shape, dtype, dev)
     code = _code(dtype)
+    given = out
     if out is None:
         out = torch.empty_like(x)
         po = out.data_ptr()
@@ -211,6 +227,8 @@ def dropout(x, rate: float, seed: int, stream: int = 0, offset: int = 0, residua
         po = _tensor("out", out, shape, dtype, dev)
     check(_L.gtmoe_dropout(px, pr, code, x.numel(), _number("rate", rate), *_generator(seed, stream, offset), po,
                            _stream(dev)))
+    if given is not None:
+        _wrote(given)
     return out
 
 
@@ -222,6 +240,7 @@ def dropout_backward(output_gradients, rate: float, seed: int, stream: int = 0, 
     g = output_gradients
     pg, dev = _values("output_gradients", g)
     code = _code(g.dtype)
+    given = input_gradients
     if input_gradients is None:
         input_gradients = torch.empty_like(g)
         pdx = input_gradients.data_ptr()
@@ -229,6 +248,8 @@ def dropout_backward(output_gradients, rate: float, seed: int, stream: int = 0, 
         pdx = _tensor("input_gradients", input_gradients, g.shape, g.dtype, dev)
     check(_L.gtmoe_dropout_backward(pg, code, g.numel(), _number("rate", rate), *_generator(seed, stream, offset),
                                     pdx, _stream(dev)))
+    if given is not None:
+        _wrote(given)
     return input_gradients
 
 
@@ -251,12 +272,15 @@ def grouped_product(x, weights, counts, out=None):
     rows, dtype = x.shape[0], x.dtype
     pc = _tensor("counts", counts, (groups,), torch.int64, dev)
     code = _code(dtype)
+    given = out
     if out is None:
         out = torch.empty((rows, outputs), dtype=dtype, device=x.device)
         po = out.data_ptr()
     else:
         po = _tensor("out", out, (rows, outputs), dtype, dev)
     check(_L.gtmoe_grouped_product(px, pw, code, rows, inputs, outputs, groups, pc, po, _stream(dev)))
+    if given is not None:
+        _wrote(given)
     return out
 
 
@@ -268,12 +292,15 @@ def grouped_product_input_gradients(output_gradients, weights, counts, input_gra
     rows, dtype = g.shape[0], g.dtype
     pc = _tensor("counts", counts, (groups,), torch.int64, dev)
     code = _code(dtype)
+    given = input_gradients
     if input_gradients is None:
         input_gradients = torch.empty((rows, inputs), dtype=dtype, device=g.device)
         pdx = input_gradients.data_ptr()
     else:
         pdx = _tensor("input_gradients", input_gradients, (rows, inputs), dtype, dev)
     check(_L.gtmoe_grouped_product_input_grad(pg, pw, code, rows, inputs, outputs, groups, pc, pdx, _stream(dev)))
+    if given is not None:
+        _wrote(given)
     return input_gradients
 
 
@@ -307,6 +334,8 @@ def grouped_product_weight_gradients(output_gradients, x, counts, weight_grad=No
         pwork = work.data_ptr()
     check(_L.gtmoe_grouped_product_weight_grad(pg, px, code, rows, inputs, outputs, groups, pc, pdw, wcode,
                                                int(accumulate), pwork, need.value, _stream(dev)))
+    if accumulate:
+        _wrote(weight_grad)
     return weight_grad
 
 
