@@ -98,15 +98,16 @@ def _number(name: str, v):
 
 def _generator(seed, stream, offset=0):
     """The generator's arguments; of longer ones the library would see the last 64 bits."""
+    if type(seed) is type(stream) is type(offset) is int:
+        if 0 <= seed < 1 << 64 and 0 <= stream < 1 << 64 and 0 <= offset < 1 << 63:
+            return [seed, stream, offset]
     out = []
     for name, v, end in (("seed", seed, 1 << 64), ("stream", stream, 1 << 64), ("offset", offset, 1 << 63)):
-        if type(v) is not int:
-            if not isinstance(v, numbers.Integral):
-                raise ValueError(f"{name} must be a whole number, got {type(v).__name__}")
-            v = int(v)
+        if not isinstance(v, numbers.Integral):
+            raise ValueError(f"{name} must be a whole number, got {type(v).__name__}")
         if not -(1 << 63) <= v < end:
             raise ValueError(f"{name} must be a number of 64 bits, got {v}")
-        out.append(v)
+        out.append(int(v))
     return out
 
 
