@@ -33,14 +33,18 @@
 // sum made in one accumulator comes out short, by more the longer it is.
 // Measured: float32 results of normal values 4.0e-7 over 512 terms and 6.2e-7
 // over 768 (a float32 sum with rounding errs by 2e-7 to 4e-7, to both sides);
-// values of one sign 2.4e-5 over 8192 terms, 6.6e-5 over 65536, 1.6e-3 over
+// values of one sign 3e-6 over 2048 terms, 2.4e-5 over 8192, 6.6e-5 over 65536, 1.6e-3 over
 // 262144, 7.0e-3 over 1048576 (bf16's half step is 3.9e-3).  Sums are therefore
 // made in runs of stages, which the epilogue adds in registers, with rounding,
 // while the next run is multiplied.  Float32 results in runs of 512 terms: of
 // 768 they took 1.5 % less time and erred by 6.8e-7 instead of 4.5e-7; of 256
 // they took 14 % more, as the epilogue needs about five stages to add a run up.
-// Results in bf16 in runs of 8192 terms, which cost less than 1 %; products
-// whose sums are no longer than that have a kernel without the registers for it.
+// Results in bf16 in runs of 1024 terms: of 2048 terms they took up to 2 % less
+// time (8192 rows in 16 groups, 2048 -> 1024: 47.1 and 48.0 us) and 1.1e-3 of
+// the values were rounded to another bf16 number than the exact sum, instead of
+// 6.2e-4; of 512 terms 3 % more, and 3.2e-4 (a float32 sum with rounding:
+// 2.5e-4).  Products whose sums have one run at most have a kernel without the
+// registers for more.
 // Every 16 runs join a total in local memory, and what that addition rounds off
 // is carried on (fold(), grouped.h): equal rows would otherwise be rounded
 // alike every time (1.6e-4 over 16777216 rows).
@@ -71,7 +75,7 @@ constexpr int kTileM = 2 * kHalf, kTileN = 2 * kHalf;
 constexpr int kOperandBytes = kHalf * kStageK * 2;  // 16 KB
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kRunStages = 8;            // stages per run of a float32 weight gradient's sums (512 rows)
-constexpr int kLongRunStages = 128;      // and of sums rounded to bf16 (8192 terms)
+constexpr int kLongRunStages = 16;       // and of sums rounded to bf16 (1024 terms)
 constexpr int kFoldRuns = 16;            // runs added up in a register before they join the total
 constexpr int kPartStep = 768;           // rows of a part of a group: a multiple of this
 constexpr int kChunkBytes = kStageK * 128;  // 64 columns x 64 terms of an M- or N-major operand

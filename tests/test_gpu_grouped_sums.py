@@ -3,7 +3,7 @@ they have one sign or repeat, may not show beyond each result's own precision.
 
 The tensor cores cut additions towards zero (at most 2^-23 of the sum each),
 so a sum is made in runs of stages of 64 terms, four additions to a stage: 8
-stages for float32 results, 128 for bfloat16 ones.  Runs are added with
+stages for float32 results, 16 for bfloat16 ones.  Runs are added with
 rounding, and what sixteen of them round off is carried along, so the bounds
 below are those of a run.  The SIMT cores make sums of more than 1024 terms in
 runs of 256 rounded additions and carry what every run's addition rounds off."""
@@ -43,7 +43,7 @@ def test_bfloat16_results_do_not_lean(call):
     bfloat16 err evenly to both sides, at most 2^-8 each with a deviation of at
     most 2^-8 / sqrt(3): the mean of 256 x 256 of them whose 256 row factors
     and 256 column factors are independent is within 8 deviations / 256.  The
-    cut additions of a run are at most 512 * 2^-23, half of that on average for
+    cut additions of a run are at most 64 * 2^-23, half of that on average for
     an even cut and half again because partial sums grow evenly; one sum over
     all the terms would lean by 1.6e-3 (262144 terms)."""
     n = 1 << 18 if call != "weight gradients" else 60000
@@ -60,8 +60,8 @@ def test_bfloat16_results_do_not_lean(call):
             got = moe.grouped_product(x, w[None], c)
         else:
             got = moe.grouped_product_input_gradients(x, w.T.contiguous()[None], c)
-    assert abs(lean(got, ref)) <= 8 * 2.0**-8 / 3**0.5 / 256 + 512 * 2.0**-23 / 4
-    R.within("results", got, ref.cpu(), ref.cpu().abs() * (R.HALF[BF16] + (512 + 33) * 2.0**-23))
+    assert abs(lean(got, ref)) <= 8 * 2.0**-8 / 3**0.5 / 256 + 64 * 2.0**-23 / 4
+    R.within("results", got, ref.cpu(), ref.cpu().abs() * (R.HALF[BF16] + (64 + 33) * 2.0**-23))
     moe.check_operators()
 
 
