@@ -54,10 +54,10 @@
 // coalesced rows), warp 10 loads B, warp 11 zeroes row tails.  Two accumulators: the epilogue of a tile
 // overlaps the next tile's products.  Every wait is bounded as in tc.cu.
 //
-// Measured (B200, in loops of most of a second, at the power cap): 8192^3 1302
-// TF/s (cuBLAS 1373); 64 groups of 1536 rows, 2048 x 2048, product and input
-// gradient 1217 TF/s (cuBLAS's batched product 1234), float32 weight gradient
-// 1081; 384 rows in 64 groups, 2048 -> 1408, 71.5 us = 5.2 TB/s of weights.
+// Measured (B200, in loops of most of a second, at the power cap): 8192^3 1260
+// TF/s (cuBLAS 1340); 64 groups of 1536 rows, 2048 x 2048, product and input
+// gradient 1193 TF/s (cuBLAS's batched product 1219), float32 weight gradient
+// 1056; 384 rows in 64 groups, 2048 -> 1408, 72.3 us = 5.1 TB/s of weights.
 #include <atomic>
 
 #include "grouped.h"

@@ -601,7 +601,8 @@ __global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(const 
 
 // The blocks' partial rows to the weight (blockIdx.y 0) and bias gradients: 32
 // columns per block, 32 runs of partial rows side by side, added in a fixed
-// order.  Launched while the backward still runs; it waits for its end.
+// order.  The backward gives no earlier sign than its end, so this launch only
+// hides its own set-up behind the last blocks (a sign sooner changed nothing).
 template <typename W, typename ACC>
 __global__ void __launch_bounds__(1024) norm_params_kernel(const ACC *__restrict__ partial, int blocks, int n,
                                                            void *dweight, void *dbias, int accumulate) {

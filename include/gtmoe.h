@@ -369,7 +369,8 @@ GTMOE_API int gtmoe_set_dropout(gtmoe_t h, double rate, uint64_t seed, uint64_t 
  *   dx[r] = dy[r] w_g
  *   dw_g  = sum over g's rows of dy[r]^T x[r]; in dtype, or float32 beside
  *           bfloat16; zeros for a group without rows; accumulate != 0 adds
- * All operands have one dtype; sums are float32 (float64 for float64).  At
+ * All operands have one dtype; sums are float32 (float64 for float64), long
+ * ones in runs, so that their error does not grow with their length.  At
  * most 1024 groups and 2^31 - 256 rows.  counts is device memory, so no call
  * waits for the host.  Rows after the last group's are neither read nor
  * written.  A negative count (taken as 0) or a sum above `rows` (rows past the
