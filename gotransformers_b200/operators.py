@@ -21,6 +21,7 @@ from ._lib import DTYPE_BF16, DTYPE_F32, DTYPE_F64, check
 torch = None
 _L = None
 _CODES: dict = {}
+_WORD = (1 << 64) - 1
 
 
 def _load():
@@ -89,26 +90,27 @@ def _stream(device: int) -> int:
 
 
 def _number(name: str, v):
-    if type(v) is not float:
-        if not isinstance(v, numbers.Real):
-            raise ValueError(f"{name} must be a number, got {type(v).__name__}")
-        v = float(v)
-    return v
+    if type(v) is float:
+        return v
+    try:
+        if not isinstance(v, (str, bytes, bytearray)):  # float() would read these
+            return float(v)
+    except (TypeError, ValueError):
+        pass
+    raise ValueError(f"{name} must be a number, got {type(v).__name__}")
 
 
 def _generator(seed, stream, offset=0):
-    """The generator's arguments; of longer ones the library would see the last 64 bits."""
-    if type(seed) is type(stream) is type(offset) is int:
-        if 0 <= seed < 1 << 64 and 0 <= stream < 1 << 64 and 0 <= offset < 1 << 63:
-            return [seed, stream, offset]
-    out = []
-    for name, v, end in (("seed", seed, 1 << 64), ("stream", stream, 1 << 64), ("offset", offset, 1 << 63)):
-        if not isinstance(v, numbers.Integral):
-            raise ValueError(f"{name} must be a whole number, got {type(v).__name__}")
-        if not -(1 << 63) <= v < end:
-            raise ValueError(f"{name} must be a number of 64 bits, got {v}")
-        out.append(int(v))
-    return out
+    """The generator's arguments as the library takes them: seed and stream
+    modulo 2^64, an offset that it would see only a part of refused."""
+    if not type(seed) is type(stream) is type(offset) is int:
+        for name, v in (("seed", seed), ("stream", stream), ("offset", offset)):
+            if not isinstance(v, numbers.Integral):
+                raise ValueError(f"{name} must be a whole number, got {type(v).__name__}")
+        seed, stream, offset = int(seed), int(stream), int(offset)
+    if not -(1 << 63) <= offset < 1 << 63:
+        raise ValueError(f"offset must be below 2^63, got {offset}")
+    return [seed & _WORD, stream & _WORD, offset]
 
 
 def _wrote(*given):
@@ -214,8 +216,8 @@ def layer_norm_backward(output_gradients, x, mean, rstd, weight=None, residual_g
 def dropout(x, rate: float, seed: int, stream: int = 0, offset: int = 0, residual=None, out=None):
     """residual + x * keep / (1 - rate) for a tensor of any shape.  Whether
     element i (in memory order) is kept depends on (seed, stream, offset + i)
-    alone, so dropout_backward makes the same decisions again.  `out` may be
-    x or residual."""
+    alone, seed and stream modulo 2^64, so dropout_backward makes the same
+    decisions again.  `out` may be x or residual."""
     px, dev = _values("x", x)
     shape, dtype = x.shape, x.dtype
     pr = None if residual is None else _tensor("residual", residual, shape, dtype, dev)
