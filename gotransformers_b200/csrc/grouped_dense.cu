@@ -33,10 +33,10 @@
 // sum made in one accumulator comes out short, by more the longer it is.
 // Measured: float32 results of normal values 4.0e-7 over 512 terms and 6.2e-7
 // over 768 (a float32 sum with rounding errs by 2e-7 to 4e-7, to both sides);
-// values of one sign 3e-6 over 2048 terms, 2.4e-5 over 8192, 6.6e-5 over 65536, 1.6e-3 over
-// 262144, 7.0e-3 over 1048576 (bf16's half step is 3.9e-3).  Sums are therefore
-// made in runs of stages, which the epilogue adds in registers, with rounding,
-// while the next run is multiplied.  Float32 results in runs of 512 terms: of
+// values of one sign 3e-6 over 2048 terms, 2.4e-5 over 8192, 6.6e-5 over 65536,
+// 1.6e-3 over 262144, 7.0e-3 over 1048576 (bf16's half step is 3.9e-3).  Sums
+// are therefore made in runs of stages, which the epilogue adds in registers,
+// with rounding, while the next run is multiplied.  Float32 results in runs of 512 terms: of
 // 768 they took 1.5 % less time and erred by 6.8e-7 instead of 4.5e-7; of 256
 // they took 14 % more, as the epilogue needs about five stages to add a run up.
 // Results in bf16 in runs of 1024 terms: of 2048 terms they took up to 2 % less
